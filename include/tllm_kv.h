@@ -257,6 +257,77 @@ int tl_sample_tokens(const void *logits, long long row_stride, int rows, int voc
                      float temperature, int top_k, float top_p, unsigned long long seed, unsigned long long step,
                      int *tokens_out, tl_stream_t stream);
 
+/* Element types of tl_token_logprobs' logits. */
+enum tl_dtype { TL_F16 = 0, TL_BF16 = 1, TL_F32 = 2 };
+
+/* Log probabilities of given tokens for `rows` rows of logits (element type
+ * `dtype`, row_stride elements apart; 0 shares one row), with each row's
+ * entropy and its top_n largest alternatives: what a server answers beside a
+ * sampled token, and what scores a prompt. No reference counterpart. Of
+ * p = softmax(logits / T), T = temperature clamped to >= 1e-5 as the
+ * sampler's: logprobs[r] = log p(tokens[r]), entropy[r] = -sum p log p (both
+ * natural), top_tokens/top_logprobs [rows][top_n] the largest logits in
+ * descending order, ties by ascending index, top_n 0..64. Sums in fp32. A
+ * logit of -inf has probability 0: its log probability is -inf, it adds
+ * nothing to the entropy and is no alternative; places without one hold
+ * (-1, -inf). A row of nothing but -inf: log probability -inf, entropy 0. A
+ * row that holds a NaN or +inf: NaN, and alternatives (-1, NaN). A negative
+ * token (padding) gives 0, one >= vocab NaN. All pointers are device memory,
+ * tokens int32; logprobs, entropy and either top output may be null,
+ * though not all of them; tokens is read for logprobs alone. No handle: the call runs on the
+ * current device, errors are read with tl_last_error(NULL). */
+int tl_token_logprobs(const void *logits, int dtype, long long row_stride, int rows, int vocab, float temperature,
+                      const int *tokens, float *logprobs, float *entropy, int top_n, int *top_tokens,
+                      float *top_logprobs, tl_stream_t stream);
+
+/* ---- W8A16 projections with their epilogue ------------------------------
+ * The layer's other projections (output, gate/up, down, LM head), replacing
+ * kernels::w8a16_matmul and the elementwise kernels around it (reference
+ * kernels/w8a16_matmul.cu:119-235, called at src/transformer.cpp:246-247 and
+ * in the feed-forward), over weights packed once at load. No handle and no
+ * workspace: the calls run on the current device, which holds every buffer;
+ * calls on different streams may overlap; errors are read with
+ * tl_last_error(NULL). */
+enum tl_activation {
+    TL_ACT_NONE = 0,
+    TL_ACT_RELU = 1,
+    TL_ACT_GELU = 2,      /* v * Phi(v), with erf */
+    TL_ACT_GELU_TANH = 3, /* its tanh form */
+    TL_ACT_SILU = 4
+};
+
+/* Bytes of the packed form of a k x n weight (of a pair of them: gated != 0);
+ * 0 for a shape that is not supported (k, n positive, k <= 2^20, n <= 2^22,
+ * group_size 32, 64 or 128). */
+size_t tl_linear_packed_bytes(int k, int n, int group_size, int gated);
+/* Packs one weight once, at model load: w int8 [k][n] row-major, scales fp16
+ * [ceil(k / group_size)][n] (the reference's QuantizedWeight layout,
+ * include/tiny_llm/types.h:33-44; k need not be a multiple of the group).
+ * w_up/scales_up: the other projection of a gated pair (same shape), w then
+ * being the gate; null for a single weight. packed: device memory of
+ * tl_linear_packed_bytes, 16-byte aligned, overlapping no source.
+ * Asynchronous on `stream`. */
+int tl_linear_pack(const int8_t *w, const void *scales, const int8_t *w_up, const void *scales_up, int k, int n,
+                   int group_size, void *packed, tl_stream_t stream);
+/* y[r][c] = act(sum_i x[r][i] w[i][c] scale[i / group_size][c] + bias[c]) + residual[r][c]
+ * for `rows` rows: x fp16, rows x_stride elements apart (>= k, a multiple of
+ * 8; x 16-byte aligned), y and residual fp16, rows y_stride / residual_stride
+ * apart (>= n). bias and residual may be null; residual may be y itself.
+ * Otherwise y overlaps no input. Products and sums in fp32 (the tensor
+ * cores' accumulation), one rounding, to fp16. Any k and n >= 1, rows from 0
+ * (nothing is done) to 2^20; k, n and group_size as given to
+ * tl_linear_pack. Rows do not affect one another, and a row's result
+ * depends on neither timing nor stream. */
+int tl_linear(const void *x, long long x_stride, int rows, const void *packed, int k, int n, int group_size,
+              const void *bias, int activation, const void *residual, long long residual_stride, void *y,
+              long long y_stride, tl_stream_t stream);
+/* The gated feed-forward product, both projections in one kernel:
+ * y[r][c] = act(x W + bias)[r][c] * (x W_up + bias_up)[r][c], from a pair
+ * packed together (n: columns of each). Arguments as tl_linear's. */
+int tl_linear_gated(const void *x, long long x_stride, int rows, const void *packed, int k, int n, int group_size,
+                    const void *bias, const void *bias_up, int activation, void *y, long long y_stride,
+                    tl_stream_t stream);
+
 /* ---- Head-sharded decode across the GPUs of one node -------------------
  * No reference counterpart (the reference is single-GPU). With KV heads
  * split over `world` ranks (one process per GPU), each rank's decode writes

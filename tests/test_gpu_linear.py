@@ -1,0 +1,302 @@
+"""tl_linear and tl_linear_gated on the device against the same products in
+float64 over the dequantized weights, at the sizes where the tiles, blocks of
+K, scale groups and row blocks end inside something.
+
+Tolerance. The result is rounded once to fp16 (half a unit: 2^-11 of the
+value, 2^-25 below the normal range). Before that, products of fp16 and int8
+numbers are exact in fp32 and their sums carry, per addition, at most one fp32
+unit of the running sum (the tensor cores truncate): at most k 2^-23 of
+sum |x w s| over a row's k terms, plus the scaling's and the epilogue's few
+roundings; activations have a slope of at most 1.13 (gelu) and the given
+functions' own errors of a few units of 2^-23. A gated product multiplies two
+such numbers."""
+import math
+
+import numpy as np
+import pytest
+
+import conftest
+import tiny_llm_b200 as T
+
+pytestmark = pytest.mark.gpu
+
+U16, U32 = 2.0**-11, 2.0**-23
+
+
+@pytest.fixture(autouse=True)
+def _need_gpu():
+    if not conftest.cuda_available():
+        pytest.skip("no CUDA device")
+
+
+def act64(act, v):
+    import torch
+    F = torch.nn.functional
+    return [lambda t: t, torch.relu, F.gelu, lambda t: F.gelu(t, approximate="tanh"), F.silu][act](v)
+
+
+class Weight:
+    """int8 weight and scales on the device, their values in float64."""
+
+    def __init__(self, k, n, group, gen, scale=None):
+        import torch
+        self.w = torch.randint(-128, 128, (k, n), device="cuda", generator=gen, dtype=torch.int16).to(torch.int8)
+        s = torch.rand(-(-k // group), n, device="cuda", generator=gen) + 0.5
+        self.s = (s * (scale or 1.0 / (74.0 * math.sqrt(k)))).half()
+        self.v = self.w.double() * self.s.double().repeat_interleave(group, 0)[:k]
+
+
+def pack(k, n, group, a, b=None):
+    import torch
+    size = T.linear_packed_bytes(k, n, group, b is not None)
+    packed = torch.full((size + 64,), 0x5A, device="cuda", dtype=torch.uint8)
+    T.pack_linear_weight(a.w.data_ptr(), a.s.data_ptr(), k, n, group, packed.data_ptr(),
+                         b.w.data_ptr() if b else 0, b.s.data_ptr() if b else 0)
+    torch.cuda.synchronize()
+    assert (packed[size:] == 0x5A).all()
+    return packed[:size]
+
+
+def make_x(rows, k, gen, stride=None):
+    import torch
+    stride = stride or -(-k // 8) * 8
+    buf = torch.full((rows, stride), float("nan"), device="cuda", dtype=torch.float16)  # what lies between rows is never read into a result
+    buf[:, :k] = torch.randn(rows, k, device="cuda", generator=gen).half()
+    return buf
+
+
+def bounds(x, W, k, slope=1.13):
+    """How far sum x W may be off in fp32 sums of products."""
+    return slope * (k + 64) * U32 * (x.abs() @ W.abs())
+
+
+def run_linear(rows, k, n, group, act=0, bias=False, residual=False, seed=0, x_stride=None, y_stride=None,
+               res_stride=None, in_place=False):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(1000 + seed)
+    W = Weight(k, n, group, gen)
+    packed = pack(k, n, group, W)
+    xb = make_x(rows, k, gen, x_stride)
+    b = torch.randn(n, device="cuda", generator=gen).half() if bias else None
+    ys = y_stride or n
+    yb = torch.full((rows + 1, ys), 7.0, device="cuda", dtype=torch.float16)
+    rs = res_stride or n
+    res = torch.randn(rows, rs, device="cuda", generator=gen).half() if residual else None
+    if in_place:
+        yb[:rows, :n] = res[:, :n]
+    kept = res.clone() if residual else None
+    T.linear(xb.data_ptr(), rows, packed.data_ptr(), k, n, group, yb.data_ptr(), bias=b.data_ptr() if bias else 0,
+             activation=act, residual=(yb if in_place else res).data_ptr() if residual else 0, x_stride=xb.stride(0),
+             y_stride=ys, residual_stride=ys if in_place else rs)
+    torch.cuda.synchronize()
+    got = yb[:rows, :n]
+    x = xb[:, :k].double()
+    pre = x @ W.v + (b.double() if bias else 0)
+    ref = act64(act, pre) + (kept[:, :n].double() if residual else 0)
+    tol = bounds(x, W.v, k) + 16 * U32 * (pre.abs() + ref.abs()) + U16 * ref.abs() + 2.0**-25
+    err = (got.double() - ref).abs()
+    assert (err <= tol).all(), f"worst {((err - tol).max().item())} at {int((err - tol).argmax())}"
+    assert (yb[rows] == 7.0).all() and (yb[:rows, n:] == 7.0).all()  # nothing else is written
+    return got
+
+
+ROWS = [1, 2, 8, 9, 16, 17, 31, 32, 33, 64, 65, 100, 128, 192, 193, 257]
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_rows(rows):
+    run_linear(rows, 512, 320, 128, residual=True, seed=rows)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 32, 70])
+@pytest.mark.parametrize("k,n,group", [
+    (1, 1, 128), (7, 3, 32), (8, 64, 64), (31, 65, 32), (33, 129, 32), (64, 127, 64), (65, 128, 64), (127, 63, 128),
+    (128, 200, 128), (129, 1, 128), (255, 77, 32), (1000, 333, 128), (1003, 1001, 64), (4096, 64, 128), (5000, 130, 32),
+])
+def test_odd_sizes(rows, k, n, group):
+    run_linear(rows, k, n, group, act=(k + n) % 5, bias=k % 2 == 1, residual=n % 2 == 1, seed=k * 7 + n)
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("act", range(5))
+@pytest.mark.parametrize("bias", [False, True])
+def test_epilogues(rows, act, bias):
+    run_linear(rows, 300, 200, 64, act=act, bias=bias, residual=True, seed=act)
+
+
+@pytest.mark.parametrize("rows", [4, 48])
+def test_strides_and_in_place_residual(rows):
+    run_linear(rows, 200, 100, 32, residual=True, x_stride=264, y_stride=111, res_stride=103, seed=1)
+    run_linear(rows, 200, 100, 32, residual=True, in_place=True, y_stride=105, seed=2)
+    run_linear(rows, 200, 104, 32, residual=True, y_stride=112, res_stride=120, seed=3)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 20, 33, 130, 200])
+@pytest.mark.parametrize("k,n,group", [(256, 64, 128), (129, 33, 64), (1000, 77, 32), (2048, 500, 128), (40, 1, 32)])
+@pytest.mark.parametrize("act,bias", [(4, False), (2, True)])
+def test_gated(rows, k, n, group, act, bias):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(k + n + rows)
+    A, B = Weight(k, n, group, gen), Weight(k, n, group, gen)
+    packed = pack(k, n, group, A, B)
+    xb = make_x(rows, k, gen)
+    ba, bb = (torch.randn(n, device="cuda", generator=gen).half() for _ in range(2))
+    y = torch.full((rows + 1, n + 3), 7.0, device="cuda", dtype=torch.float16)
+    T.linear_gated(xb.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr(), activation=act,
+                   bias=ba.data_ptr() if bias else 0, bias_up=bb.data_ptr() if bias else 0, x_stride=xb.stride(0),
+                   y_stride=n + 3)
+    torch.cuda.synchronize()
+    x = xb[:, :k].double()
+    g = x @ A.v + (ba.double() if bias else 0)
+    u = x @ B.v + (bb.double() if bias else 0)
+    ag = act64(act, g)
+    ref = ag * u
+    eg = bounds(x, A.v, k) + 16 * U32 * g.abs()
+    eu = bounds(x, B.v, k, 1.0) + 2 * U32 * u.abs()
+    tol = eg * u.abs() + eu * ag.abs() + eg * eu + 4 * U32 * ref.abs() + U16 * ref.abs() + 2.0**-25
+    err = (y[:rows, :n].double() - ref).abs()
+    assert (err <= tol).all(), f"worst {((err - tol).max().item())}"
+    assert (y[rows] == 7.0).all() and (y[:rows, n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("rows", [3, 40, 300])
+def test_rows_are_independent(rows):
+    """NaN and infinities of one row stay in it; a row's result does not
+    depend on the rows beside it or on the run."""
+    import torch
+    k, n, group = 700, 150, 64
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    W = Weight(k, n, group, gen)
+    packed = pack(k, n, group, W)
+    x = make_x(rows, k, gen, 704)
+    y = torch.empty(3, rows, n, device="cuda", dtype=torch.float16)
+    call = lambda xx, i: T.linear(xx.data_ptr(), rows, packed.data_ptr(), k, n, group, y[i].data_ptr(), x_stride=704)  # noqa: E731
+    call(x, 0)
+    call(x, 1)
+    bad = x.clone()
+    bad[1, 3] = float("nan")
+    bad[2, 699] = float("inf")
+    call(bad, 2)
+    torch.cuda.synchronize()
+    assert torch.equal(y[0].view(torch.int16), y[1].view(torch.int16))
+    assert y[2, 1].isnan().all() and not y[2, 2].isfinite().any()
+    keep = [r for r in range(rows) if r not in (1, 2)]
+    assert torch.equal(y[0, keep], y[2, keep])
+
+
+def test_overflow_goes_to_infinity():
+    import torch
+    k, n, group = 256, 64, 128
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    W = Weight(k, n, group, gen, scale=0.05)
+    W.w.fill_(127)
+    packed = pack(k, n, group, W)
+    x = torch.full((40, k), 100.0, device="cuda", dtype=torch.float16)
+    y = torch.empty(40, n, device="cuda", dtype=torch.float16)
+    for rows in (2, 40):
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr())
+        assert (y[:rows] == float("inf")).all()
+
+
+@pytest.mark.parametrize("rows", [1, 33])
+def test_streams_and_graphs(rows):
+    """Two calls at once on two streams, and a captured call replayed on new
+    activations, give what single calls give."""
+    import torch
+    k, n, group = 4096, 512, 128
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    W = Weight(k, n, group, gen)
+    packed = pack(k, n, group, W)
+    xs = [make_x(rows, k, gen) for _ in range(2)]
+    ref = [torch.empty(rows, n, device="cuda", dtype=torch.float16) for _ in range(2)]
+    for x, y in zip(xs, ref):
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    out = [torch.empty(20, rows, n, device="cuda", dtype=torch.float16) for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for s, x, y in zip(streams, xs, out):
+            T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y[i].data_ptr(), stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for y, r in zip(out, ref):
+        assert all(torch.equal(y[i], r) for i in range(20))
+    x, y = xs[0].clone(), torch.empty_like(ref[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr(),
+                     stream=torch.cuda.current_stream().cuda_stream)
+    for i in (1, 0):
+        x.copy_(xs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ref[i])
+
+
+def test_pack_then_product_on_one_stream():
+    """The product right behind the packing of its weight, without a wait."""
+    import torch
+    k, n, group = 2048, 2048, 128
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    weights = [Weight(k, n, group, gen) for _ in range(4)]
+    x = make_x(4, k, gen)
+    packed = torch.zeros(T.linear_packed_bytes(k, n, group), device="cuda", dtype=torch.uint8)
+    y = torch.empty(4, 4, n, device="cuda", dtype=torch.float16)
+    torch.cuda.synchronize()
+    for i, W in enumerate(weights):  # one buffer, packed again between the products
+        T.pack_linear_weight(W.w.data_ptr(), W.s.data_ptr(), k, n, group, packed.data_ptr())
+        T.linear(x.data_ptr(), 4, packed.data_ptr(), k, n, group, y[i].data_ptr())
+    torch.cuda.synchronize()
+    for i, W in enumerate(weights):
+        again = pack(k, n, group, W)
+        z = torch.empty(4, n, device="cuda", dtype=torch.float16)
+        T.linear(x.data_ptr(), 4, again.data_ptr(), k, n, group, z.data_ptr())
+        torch.cuda.synchronize()
+        assert torch.equal(y[i], z)
+
+
+def test_a_layers_end_and_the_head():
+    """Output projection with its residual, gated product, down projection
+    with its residual, LM head, log probabilities and sampling of the same
+    logits, as a decode step runs them: every step against float64 on the
+    step's own (fp16) input."""
+    import torch
+    rows, hidden, inter, vocab, group = 6, 256, 688, 1003, 64
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    mats = {m: Weight(a, b, group, gen) for m, a, b in
+            [("o", hidden, hidden), ("g", hidden, inter), ("u", hidden, inter), ("d", inter, hidden), ("head", hidden, vocab)]}
+    po, pd, ph = (pack(*mats[m].w.shape, group, mats[m]) for m in ("o", "d", "head"))
+    pg = pack(hidden, inter, group, mats["g"], mats["u"])
+    attn, h = make_x(rows, hidden, gen), make_x(rows, hidden, gen)
+    h0 = h.clone()
+    mid = torch.empty(rows, inter, device="cuda", dtype=torch.float16)
+    stride = 1008
+    logits = torch.empty(rows, stride, device="cuda", dtype=torch.float16)
+    tokens = torch.empty(rows, device="cuda", dtype=torch.int32)
+    lp, ent = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    T.linear(attn.data_ptr(), rows, po.data_ptr(), hidden, hidden, group, h.data_ptr(), residual=h.data_ptr())
+    torch.cuda.synchronize()
+    h1 = h.clone()
+    T.linear_gated(h.data_ptr(), rows, pg.data_ptr(), hidden, inter, group, mid.data_ptr())
+    T.linear(mid.data_ptr(), rows, pd.data_ptr(), inter, hidden, group, h.data_ptr(), residual=h.data_ptr())
+    T.linear(h.data_ptr(), rows, ph.data_ptr(), hidden, vocab, group, logits.data_ptr(), y_stride=stride)
+    T.sample_tokens(logits.data_ptr(), stride, rows, vocab, tokens.data_ptr())
+    T.token_logprobs(logits.data_ptr(), rows, vocab, tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(), row_stride=stride)
+    torch.cuda.synchronize()
+
+    def near(got, ref, tol):
+        assert ((got.double() - ref).abs() <= tol + U16 * ref.abs() + 2.0**-25).all()
+
+    near(h1, attn.double() @ mats["o"].v + h0.double(), bounds(attn.double(), mats["o"].v, hidden) + 4 * U32)
+    g, u = h1.double() @ mats["g"].v, h1.double() @ mats["u"].v
+    e = bounds(h1.double(), mats["g"].v, hidden) + 16 * U32 * g.abs()
+    e2 = bounds(h1.double(), mats["u"].v, hidden)
+    near(mid, act64(4, g) * u, e * u.abs() + e2 * g.abs() + e * e2)
+    near(h, mid.double() @ mats["d"].v + h1.double(), bounds(mid.double(), mats["d"].v, inter) + 4 * U32 * h1.abs().double())
+    near(logits[:, :vocab], h.double() @ mats["head"].v, bounds(h.double(), mats["head"].v, hidden))
+    logp = torch.log_softmax(logits[:, :vocab].double(), 1)
+    assert torch.equal(logits.gather(1, tokens.long()[:, None])[:, 0], logits[:, :vocab].max(1).values)
+    assert ((lp.double() - logp.max(1).values).abs() < 4e-6).all()
+    assert ((ent.double() + (logp.exp() * logp).sum(1)).abs() < 4e-5).all()
+    assert np.isfinite(h.float().cpu().numpy()).all()

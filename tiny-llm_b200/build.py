@@ -31,12 +31,12 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-r
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-parameter"]
 
 CU_SOURCES = ["kv_append.cu", "paged_decode.cu", "paged_prefill_tc.cu", "qkv_append.cu", "qkv_append_tc.cu",
-              "sampling.cu", "decode_static_scratch.cu"]
-CPP_SOURCES = ["paged_kv.cpp"]
+              "sampling.cu", "decode_static_scratch.cu", "linear.cu", "logprobs.cu"]
+CPP_SOURCES = ["paged_kv.cpp", "linear_api.cpp"]
 # The C++ facade (tiny_llm::KVCacheManager) is compiled by its user, with the
 # user's include paths; the library itself exports only the C-ABI.
 FACADE_SOURCE = CSRC / "kv_cache_manager.cpp"
-HEADERS = ["kernels.h", "paged_kv.h", "ptx.cuh"]
+HEADERS = ["kernels.h", "paged_kv.h", "ptx.cuh", "linear_pack.cuh"]
 
 
 def _run(cmd: list[str]) -> None:

@@ -232,5 +232,41 @@ cudaError_t launch_qkv_append_tc(const QkvArgs &a, cudaStream_t s);
 // 2-D TMA load with 128-byte swizzle leaves the same tile in shared memory.
 cudaError_t launch_qkv_pack_weight(const int8_t *w, int K, int n, int8_t *out, cudaStream_t s);
 
+// One W8A16 projection (or gated pair) of `rows` activation rows, the weights
+// packed as linear_pack.cuh says; no workspace.
+struct LinearArgs {
+    const void *x;            // fp16 [rows][k], rows x_stride elements apart (a multiple of 8)
+    long long x_stride;
+    const void *packed;
+    int rows, k, n;           // n: output columns
+    int group;                // rows of K per scale: 32, 64 or 128
+    int gated, act;           // act: enum tl_activation
+    const void *bias, *bias2;  // fp16 [n] or nullptr; bias2: the gated pair's second projection
+    const void *residual;     // fp16 [rows][n] or nullptr
+    long long residual_stride;
+    void *y;                  // fp16 [rows][n]
+    long long y_stride;
+    int csplit;               // CTAs of a cluster that share K (set by the launcher)
+};
+cudaError_t launch_linear(LinearArgs a, int num_sms, cudaStream_t s);
+// w2/s2: the other projection of a gated pair, or nullptr.
+cudaError_t launch_linear_pack(const int8_t *w, const void *s, const int8_t *w2, const void *s2, int k, int n, int group,
+                               void *out, cudaStream_t st);
+
+// Log probabilities of one given token per row, entropy and alternatives.
+constexpr int kLogprobMaxTop = 64;
+struct LogprobArgs {
+    const void *logits;
+    long long row_stride;     // elements
+    int rows, vocab, top;
+    float inv_temperature;    // 1 / T
+    float scale_log2;         // log2(e) / T
+    const int *tokens;        // device [rows], read when logprobs is set
+    float *logprobs, *entropy;          // [rows], each optional
+    int *top_tokens;                    // [rows][top]
+    float *top_logprobs;
+    int split;                // CTAs of a cluster that share a row (set by the launcher)
+};
+cudaError_t launch_logprobs(LogprobArgs a, int dtype, int num_sms, cudaStream_t s);
 
 }  // namespace tllm

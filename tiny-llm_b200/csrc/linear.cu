@@ -1,0 +1,357 @@
+// W8A16 projections with their epilogue, for few rows (a decode step):
+//   y[r][n] = act(sum_k x[r][k] w[k][n] s[k / group][n] + bias[n]) + residual[r][n]
+// and the gated pair act(gate) * up, sm_100a. The weights are packed once
+// (linear_pack.cuh); tl_linear sends larger batches to linear_tc.cu.
+//
+// Every weight is read once per 32 rows, so the weight stream bounds it. A
+// CTA owns one tile of 64 packed columns and a range of 128-row blocks of K
+// (the whole K, or one of the equal parts that the CTAs of a cluster share).
+// A producer warp streams units (weights, scales and the rows' activations
+// of the block) through a ring of shared-memory stages with bulk copies, so
+// the bytes in flight are the ring's and hold no registers; eight consumer
+// warps take the units in turn. The weights are the A side of
+// mma.sync.m16n8k16, the batch rows the N side in blocks of 8, so a lane's
+// 16-byte chunk of weights feeds four MMA steps and no transposition is
+// needed. int8 -> fp16 is exact and the scales multiply fp32 sums of at most
+// 64 products, so no weight is rounded. tcgen05 is not used here: one UMMA
+// covers 16 rows of K whatever the batch and takes longer to issue than the
+// bytes it consumes take to arrive.
+//
+// The warps' sums meet in shared memory and, when K is split, the CTAs' in
+// distributed shared memory, both in a fixed order: the result does not
+// depend on timing. Waits are bounded; a CTA whose wait gives up writes NaN.
+#include <algorithm>
+#include <atomic>
+#include <cooperative_groups.h>
+#include <cstdint>
+#include <cuda_fp16.h>
+
+#include "kernels.h"
+#include "linear_pack.cuh"
+#include "ptx.cuh"
+
+namespace tllm {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kConsumers = 8;                      // warps
+constexpr int kThreads = 32 * (kConsumers + 1);    // + the producer warp
+constexpr int kMaxUnit = lin::unit_bytes(32);      // 8704
+constexpr int kXRow = 320;                         // bytes of a row's block of activations in a stage: 256, padded
+                                                   // so that the 8 lanes of a phase read 8 different banks
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+template <int RB>
+struct Cfg {
+    static constexpr int kStage = kMaxUnit + 8 * RB * kXRow;
+    static constexpr int kBudget = RB >= 4 ? 200 * 1024 : 104 * 1024;  // one or two CTAs per SM
+    static constexpr int kNS = kBudget / kStage;
+    static constexpr int kRowF = lin::kTileN + 4;                        // floats of a row of sums (banks)
+    static constexpr int kSumBytes = kConsumers * 8 * RB * kRowF * 4;    // every warp's sums, over the ring
+    static constexpr int kRing = kNS * kStage;
+    static constexpr int kPart = 8 * RB * kRowF * 4;                     // the CTA's sums
+    static constexpr int kSmem = kRing + kPart + 2 * kNS * 8 + 16;
+    static_assert(kSumBytes <= kRing, "the sums outgrow the ring");
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+template <int RB, bool G32>
+__global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const __grid_constant__ LinearArgs a) {
+    using C = Cfg<RB>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    float *part = reinterpret_cast<float *>(smem + C::kRing);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing + C::kPart);
+    const uint32_t full_u = ptx::smem_u32(bars), empty_u = full_u + 8 * C::kNS;
+    __shared__ int s_failed;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int csplit = a.csplit, rank = blockIdx.x % csplit, tile = blockIdx.x / csplit;
+    const int row0 = blockIdx.y * 8 * RB, nrows = min(8 * RB, a.rows - row0);
+    const int nblocks = lin::blocks(a.k);
+    const int b0 = (int)((long long)rank * nblocks / csplit), b1 = (int)((long long)(rank + 1) * nblocks / csplit);
+    const int count = b1 - b0;
+    const int unit = lin::unit_bytes(a.group);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kNS; ++s) {
+            ptx::mbar_init(full_u + 8 * s, 1);
+            ptx::mbar_init(empty_u + 8 * s, 1);
+        }
+        ptx::fence_barrier_init();
+        s_failed = 0;
+    }
+    __syncthreads();
+    ptx::griddep_launch_dependents();
+
+    if (warp == kConsumers) {
+        // ---- producer: lane 0 the unit's weights, lane r row r's activations ----
+        ptx::griddep_wait();
+        const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)tile * nblocks + b0) * unit;
+        const __half *x = static_cast<const __half *>(a.x) + (long long)(row0 + lane) * a.x_stride;
+        const uint64_t once = ptx::l2_policy_evict_first(), keep = ptx::l2_policy_evict_last();
+        int issued = 0;
+        for (int i = 0; i < count; ++i, ++issued) {
+            const int s = i % C::kNS;
+            if (i >= C::kNS && !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(
+                                                            empty_u + 8 * s, (uint32_t)((i / C::kNS - 1) & 1), kWaitNs))) {
+                s_failed = 1;
+                break;
+            }
+            const int k0 = (b0 + i) * lin::kBlockK;
+            const uint32_t xb = (uint32_t)(min(lin::kBlockK, a.k - k0) / 8) * 16u;  // whole 16-byte chunks
+            const uint32_t dst = ptx::smem_u32(smem + s * C::kStage), bar = full_u + 8 * s;
+            if (lane == 0) {
+                ptx::mbar_arrive_expect_tx(bar, (uint32_t)unit + (uint32_t)nrows * xb);
+                ptx::bulk_load(dst, w + (long long)i * unit, (uint32_t)unit, bar, once);
+            }
+            __syncwarp();
+            if (lane < nrows && xb > 0) ptx::bulk_load(dst + kMaxUnit + lane * kXRow, x + k0, xb, bar, keep);
+        }
+        if (issued < count)  // gave up: the copies in flight land (or a bounded wait passes) before the CTA goes on
+            for (int i = max(0, issued - C::kNS); i < issued; ++i)
+                ptx::mbar_wait_bounded(full_u + 8 * (i % C::kNS), (uint32_t)((i / C::kNS) & 1), kWaitNs);
+    } else {
+        // ---- consumers: warp w takes units w, w + 8, ... ----
+        const int gid = lane >> 2, tig = lane & 3;
+        float acc[4][RB][4];
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nb][rb][e] = 0.f;
+        bool ok = true;
+        for (int i = warp; i < count; i += kConsumers) {
+            const int s = i % C::kNS;
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(full_u + 8 * s, (uint32_t)((i / C::kNS) & 1), kWaitNs));
+            if (!ok) break;
+            uint8_t *st = smem + s * C::kStage;
+            const int nk = a.k - (b0 + i) * lin::kBlockK;
+            if (nk < lin::kBlockK) {  // the last block of K: what the whole chunks left out, then zeros
+                const int n8 = nk & ~7;
+                ptx::griddep_wait();
+                for (int j = lane; j < nrows * (lin::kBlockK - n8); j += 32) {
+                    const int r = j / (lin::kBlockK - n8), e = n8 + j % (lin::kBlockK - n8);
+                    const __half *x = static_cast<const __half *>(a.x) + (long long)(row0 + r) * a.x_stride +
+                                      (long long)(b0 + i) * lin::kBlockK;
+                    reinterpret_cast<__half *>(st + kMaxUnit + r * kXRow)[e] = e < nk ? x[e] : __half(0.f);
+                }
+                __syncwarp();
+            }
+            const __half *sc = reinterpret_cast<const __half *>(st + 2 * lin::kHalfBytes);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t xf[RB][8];  // rows gid of each block of 8: k 8 tig..+7 and 32 + 8 tig..+7 of the half
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const uint8_t *p = st + kMaxUnit + (rb * 8 + gid) * kXRow + h * 128 + tig * 16;
+                    const uint4 v0 = *reinterpret_cast<const uint4 *>(p);
+                    const uint4 v1 = *reinterpret_cast<const uint4 *>(p + 64);
+                    xf[rb][0] = v0.x; xf[rb][1] = v0.y; xf[rb][2] = v0.z; xf[rb][3] = v0.w;
+                    xf[rb][4] = v1.x; xf[rb][5] = v1.y; xf[rb][6] = v1.z; xf[rb][7] = v1.w;
+                }
+                const uint8_t *wp = st + h * lin::kHalfBytes + tig * 1024;
+#pragma unroll
+                for (int nb = 0; nb < 4; ++nb) {
+                    const int c0 = nb * 16 + gid;
+                    const uint4 w0 = *reinterpret_cast<const uint4 *>(wp + (c0 ^ (2 * tig)) * 16);
+                    const uint4 w1 = *reinterpret_cast<const uint4 *>(wp + ((c0 + 8) ^ (2 * tig)) * 16);
+                    const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
+                    float d[RB][4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j == 0 || (G32 && j == 2)) {
+#pragma unroll
+                            for (int rb = 0; rb < RB; ++rb) d[rb][0] = d[rb][1] = d[rb][2] = d[rb][3] = 0.f;
+                        }
+                        uint32_t a0, a1, a2, a3;
+                        lin::to_h4(u0[j], a0, a2);
+                        lin::to_h4(u1[j], a1, a3);
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb)
+                            ptx::mma_16816(d[rb], a0, a1, a2, a3, xf[rb][2 * j], xf[rb][2 * j + 1]);
+                        if (j == 3 || (G32 && j == 1)) {
+                            const int g = G32 ? 2 * h + (j >> 1) : h * 64 / a.group;
+                            const float s0 = __half2float(sc[g * lin::kTileN + c0]);
+                            const float s1 = __half2float(sc[g * lin::kTileN + c0 + 8]);
+#pragma unroll
+                            for (int rb = 0; rb < RB; ++rb) {
+                                acc[nb][rb][0] = fmaf(d[rb][0], s0, acc[nb][rb][0]);
+                                acc[nb][rb][1] = fmaf(d[rb][1], s0, acc[nb][rb][1]);
+                                acc[nb][rb][2] = fmaf(d[rb][2], s1, acc[nb][rb][2]);
+                                acc[nb][rb][3] = fmaf(d[rb][3], s1, acc[nb][rb][3]);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(empty_u + 8 * s);
+        }
+        if (!ok) s_failed = 1;
+        ptx::named_barrier_sync(1, 32 * kConsumers);  // every unit consumed: the sums go over the ring
+        float *sum = reinterpret_cast<float *>(smem) + warp * 8 * RB * C::kRowF;
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                float *p = sum + (rb * 8 + 2 * tig) * C::kRowF + nb * 16 + gid;
+                p[0] = acc[nb][rb][0];
+                p[C::kRowF] = acc[nb][rb][1];
+                p[8] = acc[nb][rb][2];
+                p[C::kRowF + 8] = acc[nb][rb][3];
+            }
+        ptx::named_barrier_sync(1, 32 * kConsumers);
+        const float *all = reinterpret_cast<const float *>(smem);
+        const int c = threadIdx.x & 63;
+#pragma unroll
+        for (int r = threadIdx.x >> 6; r < 8 * RB; r += 4) {
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < kConsumers; ++w) v += all[(w * 8 * RB + r) * C::kRowF + c];
+            part[r * C::kRowF + c] = v;
+        }
+    }
+
+    // ---- the CTAs' parts of K, in rank order, and the epilogue ----
+    __syncthreads();
+    if (s_failed) {  // a wait gave up: NaN, not a wrong number
+        for (int i = threadIdx.x; i < 8 * RB * C::kRowF; i += kThreads) part[i] = __int_as_float(0x7fffffff);
+        __syncthreads();
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    if (csplit > 1) cluster.sync();
+    ptx::griddep_wait();
+    auto total = [&](int r, int c) {
+        if (csplit == 1) return part[r * C::kRowF + c];
+        float v = 0.f;
+        for (int q = 0; q < csplit; ++q) v += *cluster.map_shared_rank(part + r * C::kRowF + c, q);
+        return v;
+    };
+    const int oc = a.gated ? lin::kTileN / 2 : lin::kTileN;  // output columns of the tile
+    const __half *bias = static_cast<const __half *>(a.bias), *bias2 = static_cast<const __half *>(a.bias2);
+    for (int i = rank * kThreads + threadIdx.x; i < nrows * oc; i += csplit * kThreads) {
+        const int r = i / oc, c = i % oc;
+        const long long n = (long long)tile * oc + c;
+        if (n >= a.n) continue;
+        float v;
+        if (a.gated) {
+            const int p = (c >> 3) * 16 + (c & 7);
+            float g = total(r, p), u = total(r, p + 8);
+            if (bias) g += __half2float(bias[n]);
+            if (bias2) u += __half2float(bias2[n]);
+            v = lin::activate(a.act, g) * u;
+        } else {
+            v = total(r, c);
+            if (bias) v += __half2float(bias[n]);
+            v = lin::activate(a.act, v);
+            if (a.residual)
+                v += __half2float(static_cast<const __half *>(a.residual)[(long long)(row0 + r) * a.residual_stride + n]);
+        }
+        static_cast<__half *>(a.y)[(long long)(row0 + r) * a.y_stride + n] = __float2half_rn(v);
+    }
+    if (csplit > 1) cluster.sync();  // no CTA leaves while another may still read its shared memory
+}
+
+// One thread per 16-byte chunk (and, past those, per scale) of the packed
+// weights. Runs once per weight at load; no tuning.
+__global__ void linear_pack_kernel(const int8_t *w, const __half *s, const int8_t *w2, const __half *s2, int k, int n,
+                                   int group, uint8_t *out) {
+    const bool gated = w2 != nullptr;
+    const int unit = lin::unit_bytes(group), nblocks = lin::blocks(k);
+    const int per = 512 + lin::kTileN * (lin::kBlockK / group);  // chunks and scales of a unit
+    const long long total = lin::tiles(n, gated) * nblocks * per;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long u = i / per;
+        const int j = (int)(i % per);
+        const long long tile = u / nblocks;
+        const int block = (int)(u % nblocks);
+        const int c = j & 63;
+        const long long p = tile * lin::kTileN + c;  // packed column
+        const bool up = gated && (p & 8);
+        const long long col = gated ? (p >> 4) * 8 + (p & 7) : p;
+        const int8_t *src = up ? w2 : w;
+        uint8_t *dst = out + u * unit;
+        if (j < 512) {
+            const int h = j >> 8, ch = (j >> 6) & 3;
+            uint32_t word[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t v = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const long long row = (long long)block * lin::kBlockK + h * 64 + (q >> 1) * 32 + 8 * ch + (q & 1) * 4 + e;
+                    const int b = row < k && col < n ? src[row * n + col] : 0;
+                    v |= (uint32_t)((b + 128) & 255) << (8 * e);
+                }
+                word[q] = v;
+            }
+            *reinterpret_cast<uint4 *>(dst + h * lin::kHalfBytes + ch * 1024 + (c ^ (2 * ch)) * 16) =
+                make_uint4(word[0], word[1], word[2], word[3]);
+        } else {
+            const int g = (j - 512) >> 6;
+            const long long grp = (long long)block * (lin::kBlockK / group) + g;
+            const long long row = grp * group;
+            const __half v = row < k && col < n ? (up ? s2 : s)[grp * n + col] : __half(0.f);
+            reinterpret_cast<__half *>(dst + 2 * lin::kHalfBytes)[g * lin::kTileN + c] = v;
+        }
+    }
+}
+
+template <int RB, bool G32>
+cudaError_t launch_t(const LinearArgs &a, cudaStream_t s) {
+    static std::atomic<unsigned long long> done{0};  // devices whose shared-memory limit is set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(linear_kernel<RB, G32>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<RB>::kSmem);
+        if (e != cudaSuccess) return e;
+        done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const long long ntiles = lin::tiles(a.n, a.gated != 0);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ntiles * a.csplit), (unsigned)((a.rows + 8 * RB - 1) / (8 * RB)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<RB>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.csplit;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, linear_kernel<RB, G32>, a);
+}
+
+}  // namespace
+
+cudaError_t launch_linear(LinearArgs a, int num_sms, cudaStream_t s) {
+    // K split over a cluster until the tiles fill the SMs' CTA slots, as long
+    // as every CTA keeps a unit for each of its warps.
+    const long long tiles = lin::tiles(a.n, a.gated != 0);
+    const int rb = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : 4;
+    const long long slots = (long long)num_sms * (rb >= 4 ? 1 : 2);
+    const int nblocks = lin::blocks(a.k);
+    a.csplit = 1;
+    while (a.csplit < 8 && tiles * a.csplit * 2 <= slots && nblocks / (a.csplit * 2) >= kConsumers) a.csplit *= 2;
+    const bool g32 = a.group == 32;
+    switch (rb) {
+    case 1: return g32 ? launch_t<1, true>(a, s) : launch_t<1, false>(a, s);
+    case 2: return g32 ? launch_t<2, true>(a, s) : launch_t<2, false>(a, s);
+    default: return g32 ? launch_t<4, true>(a, s) : launch_t<4, false>(a, s);
+    }
+}
+
+cudaError_t launch_linear_pack(const int8_t *w, const void *s, const int8_t *w2, const void *s2, int k, int n, int group,
+                               void *out, cudaStream_t st) {
+    linear_pack_kernel<<<148 * 8, 256, 0, st>>>(w, static_cast<const __half *>(s), w2, static_cast<const __half *>(s2), k,
+                                               n, group, static_cast<uint8_t *>(out));
+    return cudaGetLastError();
+}
+
+}  // namespace tllm

@@ -1,0 +1,403 @@
+// Log probabilities of given tokens, entropy and largest alternatives of rows
+// of logits, sm_100a. With z_j = (x_j - max x) / T and l = sum_j exp z_j:
+//   logprob(t) = z_t - log l
+//   entropy    = log l - (sum_j z_j exp z_j) / l
+//   top        = the largest x_j, equal ones by their index
+// One pass over a row: every thread keeps the maximum of its elements and,
+// relative to it, the two sums (fp32, base 2), rescaled when the maximum
+// grows, so the row is read from HBM once and nothing of it is kept; the
+// logits' bytes bound it. Rows too few to fill the machine are split over the
+// CTAs of a cluster, which join in distributed shared memory.
+//
+// The alternatives cost next to nothing in the pass: of the CTA's maxima over
+// groups of four threads the n-th largest is a lower bound of the n-th
+// largest logit, and only threads whose own maximum reaches it (about n of
+// them) can hold one of the n. Their elements are read again (from L2), the
+// ones that reach the bound are listed and ranked by counting. A list that
+// overflows (thousands of equal logits) is replaced by n searches of the
+// slice for the largest element behind the last one found.
+//
+// Sums are combined in a fixed order: a row's result does not depend on
+// timing.
+#include <algorithm>
+#include <cfloat>
+#include <cooperative_groups.h>
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kernels.h"
+#include "ptx.cuh"
+
+namespace tllm {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kGroups = kThreads / 4;  // at least kMaxTop
+constexpr int kMaxTop = kLogprobMaxTop;
+constexpr int kCand = 1024;
+constexpr int kMaxCluster = 8;
+static_assert(kGroups >= kMaxTop, "the bound needs as many groups as alternatives");
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// 16 bytes of logits: values in fp32 and their maximum (NaN if one is).
+template <typename T>
+struct Vec;
+template <>
+struct Vec<__half> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void load(const uint4 &v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            f[2 * i] = t.x;
+            f[2 * i + 1] = t.y;
+        }
+    }
+    static __device__ __forceinline__ float max(const uint4 &v) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&v);
+        const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void load(const uint4 &v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ float max(const uint4 &v) {
+        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+};
+template <>
+struct Vec<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void load(const uint4 &v, float (&f)[4]) {
+        f[0] = __uint_as_float(v.x);
+        f[1] = __uint_as_float(v.y);
+        f[2] = __uint_as_float(v.z);
+        f[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ float max(const uint4 &v) {
+        return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
+                       max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+    }
+    static __device__ __forceinline__ float to_float(float v) { return v; }
+};
+
+// Sums of a set of elements relative to their maximum m: l = sum 2^z and
+// t = sum z 2^z with z = (x - m) c, c = log2(e) / T. An empty set, and one of
+// -inf alone, has m = -inf, l = t = 0.
+struct Sums {
+    float m, l, t;
+};
+
+// Moves s to the maximum m >= s.m.
+__device__ __forceinline__ void rebase(Sums &s, float m, float c) {
+    if (m == s.m) return;
+    // s.m = -inf (nothing yet): d is held finite, l = t = 0 stay
+    const float d = fmaxf((s.m - m) * c, -1e30f), f = ptx::ex2(d);
+    s.t = f * fmaf(d, s.l, s.t);
+    s.l *= f;
+    s.m = m;
+}
+
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+    const float m = max_nan(a.m, b.m);
+    rebase(a, m, c);
+    rebase(b, m, c);
+    return {m, a.l + b.l, a.t + b.t};
+}
+
+__device__ __forceinline__ void add(Sums &s, float x, float c) {
+    // -inf (a masked logit, or one far below): 2^z = 0 and z held finite, so
+    // that z 2^z is 0 too
+    const float z = fmaxf((x - s.m) * c, -1e30f);
+    const float e = ptx::ex2(z);
+    s.l += e;
+    s.t = fmaf(e, z, s.t);
+}
+
+struct Best {
+    float v;
+    int i;
+};
+// Order of the alternatives: larger first, equal ones by index.
+__device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+
+struct Shared {
+    Sums sums[kWarps];
+    Sums cta;                 // read by the cluster
+    float gmax[kGroups];
+    float bound;
+    int count;
+    int found;                // entries of list
+    Best list[kMaxTop];       // read by the cluster
+    Best cand[kCand];         // candidates; then the cluster's lists
+    Best red[kWarps];
+};
+static_assert(kMaxCluster * kMaxTop <= kCand, "the cluster's lists fit the candidates' place");
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+    constexpr int N = Vec<T>::kN;
+    __shared__ Shared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = a.split, rank = blockIdx.x % split;
+    const int row = blockIdx.x / split;
+    const T *x = static_cast<const T *>(a.logits) + (long long)row * a.row_stride;
+    // this CTA's slice [lo, hi) of the row, and in it the 16-byte aligned part
+    const int lo = (int)((long long)rank * a.vocab / split), hi = (int)((long long)(rank + 1) * a.vocab / split);
+    const int mis = (int)((reinterpret_cast<uintptr_t>(x + lo) & 15) / sizeof(T));
+    const int head = min(hi - lo, mis ? N - mis : 0);
+    const int nvec = (hi - lo - head) / N;
+    const uint4 *xv = reinterpret_cast<const uint4 *>(x + lo + head);
+    const int tail0 = lo + head + nvec * N;  // [tail0, hi): what is left, < N elements
+    const float c = a.scale_log2;
+
+    if (tid == 0) {
+        sh.count = 0;
+        sh.bound = INFINITY;  // stays where a NaN leaves no group of the rank below
+    }
+    // elements that no vector holds: thread j < head has lo + j, thread 32 + j the tail's
+    int single = -1;
+    if (tid < head) single = lo + tid;
+    if (tid >= 32 && tid - 32 < hi - tail0) single = tail0 + tid - 32;
+
+    Sums s = {-INFINITY, 0.f, 0.f};
+    float own = -INFINITY;  // the thread's maximum
+    if (single >= 0) {
+        const float v = Vec<T>::to_float(x[single]);
+        own = v;
+        rebase(s, max_nan(fmaxf(v, -FLT_MAX), v), c);
+        add(s, v, c);
+    }
+    constexpr int kU = 4;  // vectors in flight per thread
+    for (int i0 = tid; i0 < nvec; i0 += kThreads * kU) {
+        uint4 v[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+            if (i0 + u * kThreads < nvec) v[u] = __ldg(xv + i0 + u * kThreads);
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+            if (i0 + u * kThreads < nvec) m = max_nan(m, Vec<T>::max(v[u]));
+        own = max_nan(own, m);
+        // a batch of -inf alone moves the maximum to -FLT_MAX, not to -inf:
+        // differences to it stay numbers
+        rebase(s, max_nan(s.m, max_nan(m, -FLT_MAX)), c);
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+            if (i0 + u * kThreads < nvec) {
+                float f[N];
+                Vec<T>::load(v[u], f);
+#pragma unroll
+                for (int e = 0; e < N; ++e) add(s, f[e], c);
+            }
+    }
+
+    // ---- the CTA's sums, and the bound of its alternatives ----
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Sums b = {__shfl_down_sync(0xffffffffu, s.m, o), __shfl_down_sync(0xffffffffu, s.l, o),
+                        __shfl_down_sync(0xffffffffu, s.t, o)};
+        s = join(s, b, c);
+    }
+    if (lane == 0) sh.sums[warp] = s;
+    const int top = a.top;
+    if (top > 0) {
+        float g = max_nan(own, __shfl_xor_sync(0xffffffffu, own, 1));
+        g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, 2));
+        if ((lane & 3) == 0) sh.gmax[tid >> 2] = g;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        Sums t = sh.sums[0];
+        for (int w = 1; w < kWarps; ++w) t = join(t, sh.sums[w], c);
+        sh.cta = t;
+    }
+    if (top > 0) {
+        if (tid < kGroups) {  // the group maximum of rank top - 1 (a NaN has rank 0: the row is answered with NaN)
+            const float g = sh.gmax[tid];
+            int r = 0;
+            for (int j = 0; j < kGroups; ++j) r += before(sh.gmax[j], j, g, tid);
+            if (r == top - 1) sh.bound = g;
+        }
+        __syncthreads();
+        const float bound = sh.bound;
+        auto offer = [&](float v, int i) {
+            if (v >= bound && v > -INFINITY) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < kCand) sh.cand[at] = {v, i};
+            }
+        };
+        if (single >= 0) offer(Vec<T>::to_float(x[single]), single);
+        // the whole warp reads the elements of each of its threads that may hold one
+        unsigned todo = __ballot_sync(0xffffffffu, own >= bound && own > -INFINITY);
+        while (todo) {
+            const int from = (warp << 5) + __ffs(todo) - 1;
+            todo &= todo - 1;
+            for (int i = from + lane * kThreads; i < nvec; i += 32 * kThreads) {
+                float f[N];
+                const uint4 v = __ldg(xv + i);
+                if (Vec<T>::max(v) >= bound) {
+                    Vec<T>::load(v, f);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) offer(f[e], lo + head + i * N + e);
+                }
+            }
+        }
+        __syncthreads();
+        const int count = sh.count;
+        if (count <= kCand) {
+            for (int j = tid; j < count; j += kThreads) {
+                const Best b = sh.cand[j];
+                int r = 0;
+                for (int q = 0; q < count; ++q) r += before(sh.cand[q].v, sh.cand[q].i, b.v, b.i);
+                if (r < top) sh.list[r] = b;
+            }
+            if (tid == 0) sh.found = min(count, top);
+        } else {
+            // more elements reach the bound than the list holds: the largest
+            // behind the last one found, top times
+            Best last = {INFINITY, -1};
+            for (int n = 0; n < top; ++n) {
+                Best b = {-INFINITY, 0x7fffffff};
+                for (int i = lo + tid; i < hi; i += kThreads) {
+                    const float v = Vec<T>::to_float(x[i]);
+                    if (before(last.v, last.i, v, i) && before(v, i, b.v, b.i)) b = {v, i};
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const Best d = {__shfl_xor_sync(0xffffffffu, b.v, o), __shfl_xor_sync(0xffffffffu, b.i, o)};
+                    if (before(d.v, d.i, b.v, b.i)) b = d;
+                }
+                if (lane == 0) sh.red[warp] = b;
+                __syncthreads();
+                b = sh.red[0];
+                for (int w = 1; w < kWarps; ++w)
+                    if (before(sh.red[w].v, sh.red[w].i, b.v, b.i)) b = sh.red[w];
+                __syncthreads();
+                last = b;
+                if (tid == 0) sh.list[n] = b;
+            }
+            if (tid == 0) sh.found = top;
+        }
+    } else if (tid == 0) {
+        sh.found = 0;
+    }
+    __syncthreads();
+
+    // ---- the row: rank 0 joins the cluster's sums and lists ----
+    cg::cluster_group cluster = cg::this_cluster();
+    Sums all = sh.cta;
+    int found = sh.found;
+    Best *merged = sh.list;
+    if (split > 1) {
+        cluster.sync();
+        if (rank == 0) {
+            for (int q = 1; q < split; ++q) all = join(all, *cluster.map_shared_rank(&sh.cta, q), c);
+            if (top > 0) {
+                // every list in its place of `cand`, missing entries last
+                for (int j = tid; j < split * top; j += kThreads) {
+                    const int q = j / top, n = j % top;
+                    const Shared *o = cluster.map_shared_rank(&sh, q);
+                    sh.cand[j] = n < o->found ? o->list[n] : Best{-INFINITY, 0x7fffffff};
+                }
+                __syncthreads();
+                for (int j = tid; j < split * top; j += kThreads) {
+                    const Best b = sh.cand[j];
+                    if (b.i == 0x7fffffff) continue;
+                    int r = 0;
+                    for (int q = 0; q < split * top; ++q) r += before(sh.cand[q].v, sh.cand[q].i, b.v, b.i);
+                    if (r < top) sh.list[r] = b;
+                }
+                found = 0;
+                for (int q = 0; q < split; ++q) found += cluster.map_shared_rank(&sh, q)->found;
+                found = min(found, top);
+                __syncthreads();
+            }
+        }
+    }
+    if (rank == 0) {
+        constexpr float kLn2 = 0.69314718055994531f;
+        const bool none = !(all.l > 0.f) && all.m <= -FLT_MAX;  // nothing but -inf
+        const bool bad = !(all.m <= FLT_MAX);                   // NaN or +inf
+        const float nan = __int_as_float(0x7fffffff);
+        const float log2l = log2f(all.l);
+        auto logprob = [&](float v) {
+            if (bad) return nan;
+            if (none || v == -INFINITY) return -INFINITY;
+            return (v - all.m) * a.inv_temperature - log2l * kLn2;  // the difference may reach the type's end: no log2 form
+        };
+        if (tid == 0) {
+            if (a.logprobs) {
+                const int t = a.tokens[row];
+                a.logprobs[row] = t < 0 ? 0.f : t >= a.vocab ? nan : logprob(Vec<T>::to_float(x[t]));
+            }
+            if (a.entropy) a.entropy[row] = bad ? nan : none ? 0.f : (log2l - all.t / all.l) * kLn2;
+        }
+        for (int n = tid; n < top; n += kThreads) {
+            const bool have = !bad && n < found;
+            const long long at = (long long)row * top + n;
+            if (a.top_tokens) a.top_tokens[at] = have ? merged[n].i : -1;
+            if (a.top_logprobs) a.top_logprobs[at] = bad ? nan : have ? logprob(merged[n].v) : -INFINITY;
+        }
+    }
+    if (split > 1) cluster.sync();  // no CTA leaves while rank 0 may still read its shared memory
+}
+
+template <typename T>
+cudaError_t launch_t(const LogprobArgs &a, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.rows * (unsigned)a.split);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a);
+}
+
+}  // namespace
+
+cudaError_t launch_logprobs(LogprobArgs a, int dtype, int num_sms, cudaStream_t s) {
+    if (a.rows <= 0) return cudaSuccess;
+    // Rows split over a cluster until they fill the SMs' CTA slots, as long as
+    // a thread keeps a few vectors.
+    const int per = dtype == 2 ? 4 : 8;
+    a.split = 1;
+    while (a.split < kMaxCluster && (long long)a.rows * a.split * 2 <= 2ll * num_sms &&
+           a.vocab / (a.split * 2) >= 2 * per * kThreads)
+        a.split *= 2;
+    switch (dtype) {
+    case 0: return launch_t<__half>(a, s);
+    case 1: return launch_t<__nv_bfloat16>(a, s);
+    case 2: return launch_t<float>(a, s);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace tllm

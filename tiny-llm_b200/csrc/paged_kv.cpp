@@ -6,7 +6,9 @@
 #include "paged_kv.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -139,6 +141,36 @@ void BlockPool::permute(uint64_t seed) {
 int set_error(tl_cache *c, int status, const std::string &msg) {
     if (c) c->last_error = msg;
     return status;
+}
+
+int set_thread_error(int status, const char *format, ...) noexcept {
+    char text[512];
+    va_list args;
+    va_start(args, format);
+    std::vsnprintf(text, sizeof text, format, args);
+    va_end(args);
+    try {
+        g_create_error = text;
+    } catch (...) {  // no memory for the message: the status says enough
+    }
+    return status;
+}
+
+int current_device_sms() noexcept {
+    static std::atomic<int> sms[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    const bool cached = dev >= 0 && dev < 64;
+    if (cached && (n = sms[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (cached) sms[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 }  // namespace tllm
@@ -1315,6 +1347,55 @@ int tl_sample_tokens(const void *logits, long long row_stride, int rows, int voc
     if (e != cudaSuccess) {
         cudaGetLastError();
         return fail(TL_ERR_CUDA, std::string("sampleTokens: launch failed: ") + cudaGetErrorString(e));
+    }
+    return TL_OK;
+}
+
+// Log probabilities of given tokens with entropy and alternatives, beside the
+// sampler (no reference counterpart: the reference answers token ids alone).
+int tl_token_logprobs(const void *logits, int dtype, long long row_stride, int rows, int vocab, float temperature,
+                      const int *tokens, float *logprobs, float *entropy, int top_n, int *top_tokens,
+                      float *top_logprobs, tl_stream_t stream) {
+    using tllm::set_thread_error;
+    if (rows < 0 || vocab <= 0)
+        return set_thread_error(TL_ERR_INVALID_ARG, "tokenLogprobs: rows must be >= 0 and vocab > 0");
+    if (dtype != TL_F16 && dtype != TL_BF16 && dtype != TL_F32)
+        return set_thread_error(TL_ERR_UNSUPPORTED, "tokenLogprobs: dtype must be TL_F16, TL_BF16 or TL_F32");
+    if (top_n < 0 || top_n > tllm::kLogprobMaxTop || rows > (1 << 27))
+        return set_thread_error(TL_ERR_UNSUPPORTED, "tokenLogprobs: top_n must be 0..%d and rows at most 2^27",
+                                tllm::kLogprobMaxTop);
+    if (rows == 0) return TL_OK;
+    if (!logits) return set_thread_error(TL_ERR_INVALID_ARG, "tokenLogprobs: logits is null");
+    if (logprobs && !tokens) return set_thread_error(TL_ERR_INVALID_ARG, "tokenLogprobs: tokens is null");
+    if (!logprobs && !entropy && !(top_n > 0 && (top_tokens || top_logprobs)))
+        return set_thread_error(TL_ERR_INVALID_ARG, "tokenLogprobs: every output is null");
+    if (rows > 1 && row_stride < vocab && row_stride != 0)
+        return set_thread_error(TL_ERR_INVALID_ARG,
+                                "tokenLogprobs: row_stride must be 0 (shared logits) or >= vocab");
+    auto mis = [](const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; };
+    if (mis(logits, dtype == TL_F32 ? 4 : 2) || mis(tokens, 4) || mis(logprobs, 4) || mis(entropy, 4) ||
+        mis(top_tokens, 4) || mis(top_logprobs, 4))
+        return set_thread_error(TL_ERR_INVALID_ARG, "tokenLogprobs: a pointer is not aligned to its elements");
+    const int sms = tllm::current_device_sms();
+    if (sms == 0) return set_thread_error(TL_ERR_NO_DEVICE, "tokenLogprobs: no CUDA device");
+    tllm::LogprobArgs a{};
+    a.logits = logits;
+    a.row_stride = row_stride;
+    a.rows = rows;
+    a.vocab = vocab;
+    a.top = top_tokens || top_logprobs ? top_n : 0;
+    const float t = temperature > 1e-5f ? temperature : 1e-5f;  // clamped as the sampler's
+    a.inv_temperature = 1.0f / t;
+    a.scale_log2 = 1.4426950408889634f / t;
+    a.tokens = tokens;
+    a.logprobs = logprobs;
+    a.entropy = entropy;
+    a.top_tokens = top_tokens;
+    a.top_logprobs = top_logprobs;
+    const cudaError_t e = tllm::launch_logprobs(a, dtype, sms, (cudaStream_t)stream);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return set_thread_error(TL_ERR_CUDA, "tokenLogprobs: launch failed: %s", cudaGetErrorString(e));
     }
     return TL_OK;
 }

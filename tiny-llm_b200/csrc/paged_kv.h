@@ -109,5 +109,10 @@ struct tl_cache {
 namespace tllm {
 
 int set_error(tl_cache *c, int status, const std::string &msg);
+// The calls without a handle: the message that tl_last_error(NULL) returns on
+// this thread. Never throws.
+int set_thread_error(int status, const char *format, ...) noexcept;
+// Number of SMs of the current device, 0 without one (cached per device).
+int current_device_sms() noexcept;
 
 }  // namespace tllm

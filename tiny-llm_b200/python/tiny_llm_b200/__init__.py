@@ -33,6 +33,9 @@ TL_BACKEND_HOST_BOOKKEEPING = 1
 TL_LAYOUT_TOKEN_MAJOR = 0
 TL_LAYOUT_HEAD_MAJOR = 1
 
+TL_F16, TL_BF16, TL_F32 = 0, 1, 2
+TL_ACT_NONE, TL_ACT_RELU, TL_ACT_GELU, TL_ACT_GELU_TANH, TL_ACT_SILU = range(5)
+
 # Every symbol include/tllm_kv.h declares (checked by the CPU tests).
 EXPORTED_SYMBOLS = [
     "tl_config_init", "tl_create", "tl_destroy", "tl_last_error", "tl_status_name",
@@ -46,6 +49,7 @@ EXPORTED_SYMBOLS = [
     "tl_decode_attention_peer", "tl_attention_step", "tl_prefill_attention",
     "tl_project_qkv_append", "tl_sample_tokens", "tl_set_peer_wait_limit", "tl_debug_peer_attach",
     "tl_qkv_pack_weight", "tl_project_qkv_append_packed",
+    "tl_linear_packed_bytes", "tl_linear_pack", "tl_linear", "tl_linear_gated", "tl_token_logprobs",
 ]
 
 
@@ -148,6 +152,11 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
         "tl_project_qkv_append_packed": (i, [vp, i, vp, i, vp, vp, vp, vp, vp, vp, i, ip, i, vp, vp]),
         "tl_qkv_pack_weight": (i, [vp, i, i, vp, vp]),
         "tl_sample_tokens": (i, [vp, ll, i, i, i, f, i, f, C.c_ulonglong, C.c_ulonglong, vp, vp]),
+        "tl_token_logprobs": (i, [vp, i, ll, i, i, f, vp, vp, vp, i, vp, vp, vp]),
+        "tl_linear_packed_bytes": (sz, [i, i, i, i]),
+        "tl_linear_pack": (i, [vp, vp, vp, vp, i, i, i, vp, vp]),
+        "tl_linear": (i, [vp, ll, i, vp, i, i, i, vp, i, vp, ll, vp, ll, vp]),
+        "tl_linear_gated": (i, [vp, ll, i, vp, i, i, i, vp, vp, i, vp, ll, vp]),
         "tl_sync_check": (i, [vp, vp]),
         "tl_rope_table": (None, [C.POINTER(C.c_float), C.POINTER(C.c_float), i, i, f]),
         "tl_permute_free_blocks": (i, [vp, C.c_ulonglong]),
@@ -416,6 +425,61 @@ def pack_qkv_weight(w_ptr, hidden, n, out_ptr, stream=0):
     st = lib.tl_qkv_pack_weight(w_ptr, int(hidden), int(n), out_ptr, stream or None)
     if st != TL_OK:
         raise _ERRORS.get(st, TLError)(st, lib.tl_last_error(None).decode())
+
+
+def _check_thread(lib, st):
+    if st != TL_OK:
+        raise _ERRORS.get(st, TLError)(st, lib.tl_last_error(None).decode())
+
+
+def token_logprobs(logits_ptr, rows, vocab, tokens_ptr, logprobs_ptr, entropy_ptr=0, top_n=0, top_tokens_ptr=0,
+                   top_logprobs_ptr=0, dtype=TL_F16, row_stride=None, temperature=1.0, stream=0):
+    """tl_token_logprobs: the log probability of one given token per row of
+    logits, the rows' entropy and their top_n largest alternatives, left in
+    device memory (row_stride None: rows of `vocab`; 0 shares one row)."""
+    lib = load()
+    _check_thread(lib, lib.tl_token_logprobs(
+        logits_ptr, dtype, vocab if row_stride is None else row_stride, rows, vocab, temperature, tokens_ptr,
+        logprobs_ptr, entropy_ptr, top_n, top_tokens_ptr, top_logprobs_ptr, stream))
+
+
+def linear_packed_bytes(k, n, group_size, gated=False) -> int:
+    """tl_linear_packed_bytes: size of the packed form of a k x n weight (of
+    a gated pair of them)."""
+    lib = load()
+    size = lib.tl_linear_packed_bytes(int(k), int(n), int(group_size), int(bool(gated)))
+    if size == 0:
+        raise Unsupported(TL_ERR_UNSUPPORTED, lib.tl_last_error(None).decode())
+    return size
+
+
+def pack_linear_weight(w_ptr, scales_ptr, k, n, group_size, out_ptr, w_up_ptr=0, scales_up_ptr=0, stream=0):
+    """tl_linear_pack: int8 [k][n] weights and their fp16 scales (and those of
+    the other projection of a gated pair) into the layout linear and
+    linear_gated read (out: linear_packed_bytes)."""
+    lib = load()
+    _check_thread(lib, lib.tl_linear_pack(w_ptr, scales_ptr, w_up_ptr, scales_up_ptr, int(k), int(n),
+                                          int(group_size), out_ptr, stream))
+
+
+def linear(x_ptr, rows, packed_ptr, k, n, group_size, y_ptr, bias=0, activation=TL_ACT_NONE, residual=0,
+           x_stride=None, y_stride=None, residual_stride=None, stream=0):
+    """tl_linear: act(x W + bias) + residual for `rows` fp16 rows over packed
+    W8A16 weights (strides in elements, None: rows of k or n)."""
+    lib = load()
+    _check_thread(lib, lib.tl_linear(x_ptr, k if x_stride is None else x_stride, rows, packed_ptr, k, n, group_size,
+                                     bias, activation, residual, n if residual_stride is None else residual_stride,
+                                     y_ptr, n if y_stride is None else y_stride, stream))
+
+
+def linear_gated(x_ptr, rows, packed_ptr, k, n, group_size, y_ptr, activation=TL_ACT_SILU, bias=0, bias_up=0,
+                 x_stride=None, y_stride=None, stream=0):
+    """tl_linear_gated: act(x W + bias) * (x W_up + bias_up) over a pair of
+    weights packed together."""
+    lib = load()
+    _check_thread(lib, lib.tl_linear_gated(x_ptr, k if x_stride is None else x_stride, rows, packed_ptr, k, n,
+                                           group_size, bias, bias_up, activation, y_ptr,
+                                           n if y_stride is None else y_stride, stream))
 
 
 def inject_alloc_failure(nth: int) -> None:
