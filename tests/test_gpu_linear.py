@@ -117,6 +117,14 @@ def test_odd_sizes(rows, k, n, group):
     run_linear(rows, k, n, group, act=(k + n) % 5, bias=k % 2 == 1, residual=n % 2 == 1, seed=k * 7 + n)
 
 
+@pytest.mark.parametrize("rows,k,n,group", [(1, 8192, 20000, 128), (8, 4096, 28672, 64), (12, 6000, 20000, 32),
+                                            (30, 4096, 28672, 128), (64, 4096, 20000, 64), (150, 2048, 30000, 32),
+                                            (700, 1500, 9000, 128), (2000, 700, 3500, 64)])
+def test_many_steps(rows, k, n, group):
+    """More steps than the rings hold, more tiles than CTAs."""
+    run_linear(rows, k, n, group, residual=True, seed=rows)
+
+
 @pytest.mark.parametrize("rows", [3, 40])
 @pytest.mark.parametrize("act", range(5))
 @pytest.mark.parametrize("bias", [False, True])

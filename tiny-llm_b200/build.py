@@ -31,7 +31,8 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-r
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-parameter"]
 
 CU_SOURCES = ["kv_append.cu", "paged_decode.cu", "paged_prefill_tc.cu", "qkv_append.cu", "qkv_append_tc.cu",
-              "sampling.cu", "decode_static_scratch.cu", "linear.cu", "logprobs.cu"]
+              "sampling.cu", "decode_static_scratch.cu", "linear.cu", "linear_tc.cu",
+              "logprobs.cu"]
 CPP_SOURCES = ["paged_kv.cpp", "linear_api.cpp"]
 # The C++ facade (tiny_llm::KVCacheManager) is compiled by its user, with the
 # user's include paths; the library itself exports only the C-ABI.

@@ -6,10 +6,11 @@
 // Every weight is read once per 32 rows, so the weight stream bounds it. A
 // CTA owns one tile of 64 packed columns and a range of 128-row blocks of K
 // (the whole K, or one of the equal parts that the CTAs of a cluster share).
-// A producer warp streams units (weights, scales and the rows' activations
-// of the block) through a ring of shared-memory stages with bulk copies, so
-// the bytes in flight are the ring's and hold no registers; eight consumer
-// warps take the units in turn. The weights are the A side of
+// A producer warp streams units (weights and scales by one bulk copy, the
+// rows' activations of the block by two TMA tiles, which also zero-fill past
+// K and past the last row) through a ring of shared-memory stages, so the
+// bytes in flight are the ring's and hold no registers; eight consumer warps
+// take the units in turn, each from a stage of its own. The weights are the A side of
 // mma.sync.m16n8k16, the batch rows the N side in blocks of 8, so a lane's
 // 16-byte chunk of weights feeds four MMA steps and no transposition is
 // needed. int8 -> fp16 is exact and the scales multiply fp32 sums of at most
@@ -38,28 +39,34 @@ namespace cg = cooperative_groups;
 constexpr int kConsumers = 8;                      // warps
 constexpr int kThreads = 32 * (kConsumers + 1);    // + the producer warp
 constexpr int kMaxUnit = lin::unit_bytes(32);      // 8704
-constexpr int kXRow = 320;                         // bytes of a row's block of activations in a stage: 256, padded
-                                                   // so that the 8 lanes of a phase read 8 different banks
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 template <int RB>
 struct Cfg {
-    static constexpr int kStage = kMaxUnit + 8 * RB * kXRow;
-    static constexpr int kBudget = RB >= 4 ? 200 * 1024 : 104 * 1024;  // one or two CTAs per SM
-    static constexpr int kNS = kBudget / kStage;
+    static constexpr int kXHalf = 8 * RB * 128;  // activations of 64 rows of K: [8 RB rows][128 B], swizzled
+    static constexpr int kStage = (2 * kXHalf + kMaxUnit + 1023) / 1024 * 1024;
+    // One stage per consumer warp: a warp then meets every phase of its
+    // barrier in turn (with another count it could miss one and take the
+    // phase after it for the one before).
+    static constexpr int kNS = kConsumers;
     static constexpr int kRowF = lin::kTileN + 4;                        // floats of a row of sums (banks)
     static constexpr int kSumBytes = kConsumers * 8 * RB * kRowF * 4;    // every warp's sums, over the ring
     static constexpr int kRing = kNS * kStage;
     static constexpr int kPart = 8 * RB * kRowF * 4;                     // the CTA's sums
-    static constexpr int kSmem = kRing + kPart + 2 * kNS * 8 + 16;
+    static constexpr int kSmem = 1024 + kRing + kPart + 2 * kNS * 8 + 16;
     static_assert(kSumBytes <= kRing, "the sums outgrow the ring");
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
+struct alignas(64) Map {  // a tensor map, opaque here
+    unsigned char bytes[128];
+};
+
 template <int RB, bool G32>
-__global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const __grid_constant__ LinearArgs a) {
+__global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ Map xmap) {
     using C = Cfg<RB>;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float *part = reinterpret_cast<float *>(smem + C::kRing);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing + C::kPart);
     const uint32_t full_u = ptx::smem_u32(bars), empty_u = full_u + 8 * C::kNS;
@@ -85,32 +92,31 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const
     ptx::griddep_launch_dependents();
 
     if (warp == kConsumers) {
-        // ---- producer: lane 0 the unit's weights, lane r row r's activations ----
+        // ---- producer (one lane) ----
         ptx::griddep_wait();
-        const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)tile * nblocks + b0) * unit;
-        const __half *x = static_cast<const __half *>(a.x) + (long long)(row0 + lane) * a.x_stride;
-        const uint64_t once = ptx::l2_policy_evict_first(), keep = ptx::l2_policy_evict_last();
-        int issued = 0;
-        for (int i = 0; i < count; ++i, ++issued) {
-            const int s = i % C::kNS;
-            if (i >= C::kNS && !__all_sync(0xffffffffu, ptx::mbar_wait_bounded(
-                                                            empty_u + 8 * s, (uint32_t)((i / C::kNS - 1) & 1), kWaitNs))) {
-                s_failed = 1;
-                break;
+        if (lane == 0) {
+            const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)tile * nblocks + b0) * unit;
+            const uint64_t once = ptx::l2_policy_evict_first(), keep = ptx::l2_policy_evict_last();
+            int issued = 0;
+            for (int i = 0; i < count; ++i, ++issued) {
+                const int s = i % C::kNS;
+                if (i >= C::kNS && !ptx::mbar_wait_bounded(empty_u + 8 * s, (uint32_t)((i / C::kNS - 1) & 1), kWaitNs)) {
+                    s_failed = 1;
+                    break;
+                }
+                const int k0 = (b0 + i) * lin::kBlockK;
+                const uint32_t dst = ptx::smem_u32(smem + s * C::kStage), bar = full_u + 8 * s;
+                ptx::mbar_arrive_expect_tx(bar, (uint32_t)(unit + 2 * C::kXHalf));
+                ptx::bulk_load(dst + 2 * C::kXHalf, w + (long long)i * unit, (uint32_t)unit, bar, once);
+                // (a half block past K lies wholly out of bounds: zeros)
+                ptx::tma_load_2d(dst, &xmap, bar, k0, row0, keep);
+                ptx::tma_load_2d(dst + C::kXHalf, &xmap, bar, k0 + 64, row0, keep);
             }
-            const int k0 = (b0 + i) * lin::kBlockK;
-            const uint32_t xb = (uint32_t)(min(lin::kBlockK, a.k - k0) / 8) * 16u;  // whole 16-byte chunks
-            const uint32_t dst = ptx::smem_u32(smem + s * C::kStage), bar = full_u + 8 * s;
-            if (lane == 0) {
-                ptx::mbar_arrive_expect_tx(bar, (uint32_t)unit + (uint32_t)nrows * xb);
-                ptx::bulk_load(dst, w + (long long)i * unit, (uint32_t)unit, bar, once);
-            }
-            __syncwarp();
-            if (lane < nrows && xb > 0) ptx::bulk_load(dst + kMaxUnit + lane * kXRow, x + k0, xb, bar, keep);
+            if (issued < count)  // gave up: the copies in flight land (or a bounded wait passes) before the CTA goes on
+                for (int i = max(0, issued - C::kNS); i < issued; ++i)
+                    ptx::mbar_wait_bounded(full_u + 8 * (i % C::kNS), (uint32_t)((i / C::kNS) & 1), kWaitNs);
         }
-        if (issued < count)  // gave up: the copies in flight land (or a bounded wait passes) before the CTA goes on
-            for (int i = max(0, issued - C::kNS); i < issued; ++i)
-                ptx::mbar_wait_bounded(full_u + 8 * (i % C::kNS), (uint32_t)((i / C::kNS) & 1), kWaitNs);
+        __syncwarp();
     } else {
         // ---- consumers: warp w takes units w, w + 8, ... ----
         const int gid = lane >> 2, tig = lane & 3;
@@ -126,32 +132,21 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const
             const int s = i % C::kNS;
             ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(full_u + 8 * s, (uint32_t)((i / C::kNS) & 1), kWaitNs));
             if (!ok) break;
-            uint8_t *st = smem + s * C::kStage;
-            const int nk = a.k - (b0 + i) * lin::kBlockK;
-            if (nk < lin::kBlockK) {  // the last block of K: what the whole chunks left out, then zeros
-                const int n8 = nk & ~7;
-                ptx::griddep_wait();
-                for (int j = lane; j < nrows * (lin::kBlockK - n8); j += 32) {
-                    const int r = j / (lin::kBlockK - n8), e = n8 + j % (lin::kBlockK - n8);
-                    const __half *x = static_cast<const __half *>(a.x) + (long long)(row0 + r) * a.x_stride +
-                                      (long long)(b0 + i) * lin::kBlockK;
-                    reinterpret_cast<__half *>(st + kMaxUnit + r * kXRow)[e] = e < nk ? x[e] : __half(0.f);
-                }
-                __syncwarp();
-            }
-            const __half *sc = reinterpret_cast<const __half *>(st + 2 * lin::kHalfBytes);
+            const uint8_t *st = smem + s * C::kStage;
+            const uint8_t *wst = st + 2 * C::kXHalf;
+            const __half *sc = reinterpret_cast<const __half *>(wst + 2 * lin::kHalfBytes);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t xf[RB][8];  // rows gid of each block of 8: k 8 tig..+7 and 32 + 8 tig..+7 of the half
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    const uint8_t *p = st + kMaxUnit + (rb * 8 + gid) * kXRow + h * 128 + tig * 16;
-                    const uint4 v0 = *reinterpret_cast<const uint4 *>(p);
-                    const uint4 v1 = *reinterpret_cast<const uint4 *>(p + 64);
+                    const uint8_t *p = st + h * C::kXHalf + (rb * 8 + gid) * 128;
+                    const uint4 v0 = *reinterpret_cast<const uint4 *>(p + ((tig ^ gid) << 4));
+                    const uint4 v1 = *reinterpret_cast<const uint4 *>(p + (((4 + tig) ^ gid) << 4));
                     xf[rb][0] = v0.x; xf[rb][1] = v0.y; xf[rb][2] = v0.z; xf[rb][3] = v0.w;
                     xf[rb][4] = v1.x; xf[rb][5] = v1.y; xf[rb][6] = v1.z; xf[rb][7] = v1.w;
                 }
-                const uint8_t *wp = st + h * lin::kHalfBytes + tig * 1024;
+                const uint8_t *wp = wst + h * lin::kHalfBytes + tig * 1024;
 #pragma unroll
                 for (int nb = 0; nb < 4; ++nb) {
                     const int c0 = nb * 16 + gid;
@@ -251,6 +246,7 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const
         }
         static_cast<__half *>(a.y)[(long long)(row0 + r) * a.y_stride + n] = __float2half_rn(v);
     }
+    __syncwarp();
     if (csplit > 1) cluster.sync();  // no CTA leaves while another may still read its shared memory
 }
 
@@ -325,7 +321,11 @@ cudaError_t launch_t(const LinearArgs &a, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, linear_kernel<RB, G32>, a);
+    Map xmap;
+    e = encode_tensor_map_2d(&xmap, true, a.x, (unsigned long long)a.k, (unsigned long long)a.rows,
+                             (unsigned long long)a.x_stride * 2, 64, 8 * RB);
+    if (e != cudaSuccess) return e;
+    return cudaLaunchKernelEx(&cfg, linear_kernel<RB, G32>, a, xmap);
 }
 
 }  // namespace

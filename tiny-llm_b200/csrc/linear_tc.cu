@@ -1,0 +1,481 @@
+// W8A16 projections with their epilogue on the 5th-generation tensor cores
+// (tcgen05), sm_100a: tl_linear / tl_linear_gated for more rows than
+// linear.cu takes. Same operation, same packed weights (linear_pack.cuh).
+//
+// The packed weight columns are the M side of the UMMA (128 per tile: two
+// tiles of 64 of the packed layout), a tile of up to 192 batch rows the N
+// side, K in steps of 64. The int8 weights become the fp16 A operand on the
+// way, exactly and in TMEM; their scales multiply the fp32 sums of one scale
+// group, so no weight is rounded and no fp16 copy of the weights exists in
+// HBM or shared memory. Per CTA:
+//   producer    one lane: per step two 4 KB bulk copies of packed weights and
+//               one TMA tile of activations [rows][64] (128-byte swizzle,
+//               zeros past K and the last row) into a ring of stages;
+//   converters  thread = weight column: 64 bytes from shared memory, to 64
+//               fp16, one tcgen05.st of 32 columns: the K-major A operand;
+//   MMA         one thread: four UMMAs (K = 16) per step, A in TMEM, B in
+//               shared memory, into one of two accumulators, changed with
+//               every scale group;
+//   drains      thread = weight column (TMEM lane): when a group is complete,
+//               acc += scale * sum for the thread's rows, in registers; after
+//               the last group the epilogue straight from them.
+// So the tensor cores never wait for the scaling (the other accumulator is
+// filled meanwhile) nor for a tile's epilogue: the CTAs are persistent and
+// the next tile's groups start while the last one's is written.
+//
+// Too few tiles for the SMs: a cluster's CTAs share a tile's K and add their
+// sums in distributed shared memory, in rank order. No atomics, no workspace:
+// results do not depend on timing. Waits are bounded; a CTA whose wait gives
+// up writes NaN.
+#include <algorithm>
+#include <atomic>
+#include <cooperative_groups.h>
+#include <cstdint>
+#include <cuda_fp16.h>
+
+#include "kernels.h"
+#include "linear_pack.cuh"
+#include "ptx.cuh"
+
+namespace tllm {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kM = 128;            // packed columns of a tile
+constexpr int kStepK = 64;         // rows of K per ring stage
+constexpr int kNA = 4;             // A operand stages in TMEM (32 columns each)
+constexpr int kMaxStages = 12;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+struct alignas(64) Map {  // a tensor map, opaque here
+    unsigned char bytes[128];
+};
+
+// kRows: most rows of a tile. kCW, kDW: converter and drain warps (sets of
+// four, one per TMEM lane quarter). kPerSm: CTAs per SM.
+template <int kRows_, int kCW_, int kDW_, int kPerSm_>
+struct Cfg {
+    static constexpr int kRows = kRows_, kCW = kCW_, kDW = kDW_, kPerSm = kPerSm_;
+    static constexpr int kConvSets = kCW / 4, kDrainSets = kDW / 4;
+    static constexpr int kProd = kDW + kCW, kMma = kProd + 1;  // warps
+    static constexpr int kThreads = 32 * (kDW + kCW + 2);
+    static constexpr int kAcc = kRows / kDrainSets;  // rows per drain thread
+    static constexpr uint32_t kTmemCols = 2 * kRows + kNA * 32 <= 128 ? 128 : 2 * kRows + kNA * 32 <= 256 ? 256 : 512;
+    static constexpr int kRing = (kPerSm == 2 ? 100 : 196) * 1024;
+    static constexpr int kBars = (2 * kMaxStages + 2 * kNA + 5) * 8;
+    static constexpr int kSmem = 1024 + kRing + kBars + 16;
+    static_assert(kAcc % 16 == 0 && kPerSm * kTmemCols <= 512, "tile");
+};
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                   "=r"(r[15])
+                 : "r"(taddr));
+}
+// Waits for this thread's TMEM loads; r is read after it.
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])::"memory");
+}
+
+// Tile t of the launch: bands of 16 column tiles, in a band the row tiles in
+// turn, so that the tiles in flight share both operands in L2.
+struct TilePos {
+    int nt, rt;
+};
+__device__ __forceinline__ TilePos tile_pos(int t, int ntiles, int nrt) {
+    const int band = t / (16 * nrt), left = t - band * 16 * nrt;
+    const int width = min(16, ntiles - band * 16);
+    return {band * 16 + left % width, left / width};
+}
+
+template <typename C>
+__global__ void __launch_bounds__(C::kThreads, C::kPerSm)
+    linear_tc_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ Map xmap) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing);
+    const uint32_t full_u = ptx::smem_u32(bars);           // [stages] weights and activations landed
+    const uint32_t empty_u = full_u + 8 * kMaxStages;      // [stages] converted and multiplied
+    const uint32_t afull_u = empty_u + 8 * kMaxStages;     // [kNA] A operand in TMEM
+    const uint32_t aempty_u = afull_u + 8 * kNA;           // [kNA] A operand multiplied
+    const uint32_t dfull_u = aempty_u + 8 * kNA;           // [2] a group's sums complete
+    const uint32_t dempty_u = dfull_u + 16;                // [2] ... and drained
+    const uint32_t done_u = dempty_u + 16;                 // every UMMA complete
+    __shared__ uint32_t s_tmem;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int RT = a.row_tile;  // rows of a tile, a multiple of 32
+    const int nrt = (a.rows + RT - 1) / RT;
+    const int tiles64 = (int)lin::tiles(a.n, a.gated != 0);
+    const int ntiles = (tiles64 + 1) / 2, total = ntiles * nrt;
+    const int csplit = a.csplit, rank = blockIdx.x % csplit;
+    const int nblocks = lin::blocks(a.k), unit = lin::unit_bytes(a.group);
+    // this CTA's part of K, in blocks of 128 (whole scale groups), and its steps of 64
+    const int b0 = (int)((long long)rank * nblocks / csplit), b1 = (int)((long long)(rank + 1) * nblocks / csplit);
+    const int step0 = 2 * b0, steps = min(2 * b1, (a.k + kStepK - 1) / kStepK) - step0;
+    const int gsteps = a.group >= 64 ? a.group / 64 : 1;  // steps of a group
+    const int gper = a.group == 32 ? 2 : 1;               // groups of a step
+    const int ngroups = a.group == 32 ? 2 * steps : (steps + gsteps - 1) / gsteps;
+    const int first = blockIdx.x / csplit, stride = gridDim.x / csplit;
+    const int xbytes = RT * 128, stage_bytes = xbytes + 8192;
+    const int NS = min(kMaxStages, C::kRing / stage_bytes) & ~1;  // even: a converter set meets every phase of its stages
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kMaxStages; ++s) {
+            ptx::mbar_init(full_u + 8 * s, 1);
+            ptx::mbar_init(empty_u + 8 * s, 4 + 1);  // a converter set's warps and the MMA's commit
+        }
+        for (int s = 0; s < kNA; ++s) {
+            ptx::mbar_init(afull_u + 8 * s, 4);
+            ptx::mbar_init(aempty_u + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            ptx::mbar_init(dfull_u + 8 * s, 1);
+            ptx::mbar_init(dempty_u + 8 * s, C::kDW);
+        }
+        ptx::mbar_init(done_u, 1);
+        ptx::fence_barrier_init();
+    }
+    if (warp == C::kMma) ptx::tmem_alloc(ptx::smem_u32(&s_tmem), C::kTmemCols);
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tbase = s_tmem;             // accumulators at 0 and kRows, then the A stages
+    const uint32_t acol = 2 * C::kRows;
+    ptx::griddep_launch_dependents();
+
+    if (warp >= C::kProd) {
+        if (warp == C::kProd && lane == 0) {
+            // ---- producer ----
+            ptx::prefetch_tensormap(&xmap);
+            ptx::griddep_wait();
+            const uint64_t keep = ptx::l2_policy_evict_last();
+            const uint64_t wpol = nrt > 1 ? keep : ptx::l2_policy_evict_first();  // weights: read once per row tile
+            const uint8_t *packed = static_cast<const uint8_t *>(a.packed);
+            int it = 0;
+            bool ok = true;
+            for (int t = first; t < total && ok; t += stride) {
+                const TilePos p = tile_pos(t, ntiles, nrt);
+                const bool both = 2 * p.nt + 1 < tiles64;
+                const uint8_t *w0 = packed + (long long)(2 * p.nt) * nblocks * unit;
+                const uint8_t *w1 = w0 + (long long)nblocks * unit;
+                for (int i = 0; i < steps; ++i, ++it) {
+                    const int s = it % NS;
+                    if (it >= NS && !ptx::mbar_wait_bounded(empty_u + 8 * s, (uint32_t)((it / NS - 1) & 1), kWaitNs)) {
+                        ok = false;
+                        break;
+                    }
+                    const int step = step0 + i;
+                    const long long off = (long long)(step >> 1) * unit + (step & 1) * lin::kHalfBytes;
+                    const uint32_t dst = ptx::smem_u32(smem + s * stage_bytes), bar = full_u + 8 * s;
+                    ptx::mbar_arrive_expect_tx(bar, (uint32_t)(xbytes + (both ? 2 : 1) * lin::kHalfBytes));
+                    ptx::bulk_load(dst + xbytes, w0 + off, lin::kHalfBytes, bar, wpol);
+                    if (both) ptx::bulk_load(dst + xbytes + lin::kHalfBytes, w1 + off, lin::kHalfBytes, bar, wpol);
+                    ptx::tma_load_2d(dst, &xmap, bar, step * kStepK, p.rt * RT, keep);
+                }
+            }
+            if (!ok) {
+                // the copies in flight land (or a bounded wait passes) before the CTA goes on
+                for (int i = max(0, it - NS); i < it; ++i)
+                    ptx::mbar_wait_bounded(full_u + 8 * (i % NS), (uint32_t)((i / NS) & 1), kWaitNs);
+            }
+        } else if (warp == C::kMma && lane == 0) {
+            // ---- UMMA issue ----
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(RT >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
+            const uint32_t ring_u = ptx::smem_u32(smem);
+            int it = 0, gi = 0;  // steps and groups over all tiles
+            bool ok = true;
+            for (int t = first; t < total && ok; t += stride) {
+                int in_group = 0;  // steps of the group done
+                for (int i = 0; i < steps; ++i, ++it) {
+                    const int s = it % NS, j = it % kNA;
+                    if (in_group == 0 && gi >= 2 &&
+                        !ptx::mbar_wait_bounded(dempty_u + 8 * (gi & 1), (uint32_t)((gi / 2 - 1) & 1), kWaitNs))
+                        ok = false;
+                    ok = ok && ptx::mbar_wait_bounded(full_u + 8 * s, (uint32_t)((it / NS) & 1), kWaitNs) &&
+                         ptx::mbar_wait_bounded(afull_u + 8 * j, (uint32_t)((it / kNA) & 1), kWaitNs);
+                    if (!ok) break;
+                    ptx::tc_fence_after_sync();
+                    const uint32_t xa = ring_u + (uint32_t)(s * stage_bytes);
+                    const uint32_t at = tbase + acol + (uint32_t)(j * 32);
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        if (ks == 2 && gper == 2) {  // the step's second group
+                            ptx::umma_commit(dfull_u + 8 * (gi & 1));
+                            ++gi;
+                            if (gi >= 2 &&
+                                !ptx::mbar_wait_bounded(dempty_u + 8 * (gi & 1), (uint32_t)((gi / 2 - 1) & 1), kWaitNs)) {
+                                ok = false;
+                                break;
+                            }
+                            ptx::tc_fence_after_sync();
+                        }
+                        const bool fresh = ks == 0 ? in_group == 0 : (ks == 2 && gper == 2);
+                        ptx::umma_f16_ta(tbase + (uint32_t)((gi & 1) * C::kRows), at + (uint32_t)(8 * ks),
+                                         ptx::umma_desc_sw128(xa + ks * 32, 16, 1024), idesc, fresh ? 0u : 1u);
+                    }
+                    if (!ok) break;
+                    ptx::umma_commit(aempty_u + 8 * j);
+                    ptx::umma_commit(empty_u + 8 * s);
+                    if (++in_group == gsteps || i + 1 == steps) {
+                        ptx::umma_commit(dfull_u + 8 * (gi & 1));
+                        ++gi;
+                        in_group = 0;
+                    }
+                }
+            }
+            // every UMMA issued is complete before TMEM is freed
+            ptx::umma_commit(done_u);
+            ptx::mbar_wait_bounded(done_u, 0u, kWaitNs);
+        }
+    } else if (warp >= C::kDW) {
+        // ---- converters: set c takes steps c, c + kConvSets, ... ----
+        const int set = (warp - C::kDW) >> 2, q = warp & 3;
+        const int n64 = (q & 1) * 32 + lane;
+        const uint32_t roff = (uint32_t)(xbytes + (q >> 1) * lin::kHalfBytes);
+        const int my_tiles = first < total ? (total - first + stride - 1) / stride : 0;
+        const int all = my_tiles * steps;
+        bool ok = true;
+        for (int it = set; it < all; it += C::kConvSets) {
+            const int s = it % NS, j = it % kNA;
+            ok = ptx::mbar_wait_bounded(full_u + 8 * s, (uint32_t)((it / NS) & 1), kWaitNs);
+            ok = ok && (it < kNA || ptx::mbar_wait_bounded(aempty_u + 8 * j, (uint32_t)((it / kNA - 1) & 1), kWaitNs));
+            if (!__all_sync(0xffffffffu, ok)) {
+                ok = false;
+                break;
+            }
+            ptx::tc_fence_after_sync();
+            const uint8_t *raw = smem + s * stage_bytes + roff;
+            uint32_t r[32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(raw + c * 1024 + ((n64 ^ (2 * c)) << 4));
+                lin::to_h4(v.x, r[4 * c], r[4 * c + 1]);
+                lin::to_h4(v.y, r[4 * c + 2], r[4 * c + 3]);
+                lin::to_h4(v.z, r[16 + 4 * c], r[16 + 4 * c + 1]);
+                lin::to_h4(v.w, r[16 + 4 * c + 2], r[16 + 4 * c + 3]);
+            }
+            ptx::tmem_st32(tbase + ((uint32_t)(32 * q) << 16) + acol + (uint32_t)(j * 32), r);
+            ptx::tmem_wait_st();
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                ptx::mbar_arrive(afull_u + 8 * j);
+                ptx::mbar_arrive(empty_u + 8 * s);
+            }
+        }
+    } else {
+        // ---- drains ----
+        const int q = warp & 3, set = warp >> 2;
+        const int col = 32 * q + lane;              // packed column of the tile
+        const int per = RT / C::kDrainSets;         // rows of a drain thread, a multiple of 16
+        const int row_off = set * per;
+        const uint32_t tlane = tbase + ((uint32_t)(32 * q) << 16) + (uint32_t)row_off;
+        int gi = 0;
+        bool ok = true;
+        ptx::griddep_wait();
+        for (int t = first; t < total; t += stride) {
+            const TilePos p = tile_pos(t, ntiles, nrt);
+            const int t64 = 2 * p.nt + (q >> 1);
+            const bool real = t64 < tiles64;
+            // scales of this column, one per group
+            const uint8_t *sbase = static_cast<const uint8_t *>(a.packed) + ((long long)(real ? t64 : 0) * nblocks + b0) * unit +
+                                   2 * lin::kHalfBytes + (col & 63) * 2;
+            const int gshift = a.group == 32 ? 2 : a.group == 64 ? 1 : 0;  // log2 of the groups of a block
+            auto scale_of = [&](int g) -> float {
+                const uint8_t *sp = sbase + (long long)(g >> gshift) * unit + (g & ((1 << gshift) - 1)) * (lin::kTileN * 2);
+                return __half2float(__ushort_as_half(__ldg(reinterpret_cast<const unsigned short *>(sp))));
+            };
+            uint64_t acc[C::kAcc / 2];  // pairs of rows
+#pragma unroll
+            for (int i = 0; i < C::kAcc / 2; ++i) acc[i] = 0ull;
+            float sc = scale_of(0);
+            for (int g = 0; g < ngroups; ++g, ++gi) {
+                const uint64_t s2 = ptx::f2_pack(sc, sc);
+                if (g + 1 < ngroups) sc = scale_of(g + 1);
+                if (ok)
+                    ok = __all_sync(0xffffffffu,
+                                    ptx::mbar_wait_bounded(dfull_u + 8 * (gi & 1), (uint32_t)((gi / 2) & 1), kWaitNs));
+                if (ok) {
+                    ptx::tc_fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < C::kAcc / 16; ++c) {
+                        if (c * 16 < per) {
+                            uint32_t v[16];
+                            tmem_ld16(tlane + (uint32_t)((gi & 1) * C::kRows + c * 16), v);
+                            tmem_wait_ld16(v);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                acc[c * 8 + i] = ptx::f2_fma(
+                                    ptx::f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), s2,
+                                    acc[c * 8 + i]);
+                        }
+                    }
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(dempty_u + 8 * (gi & 1));
+                }
+            }
+            if (!ok) {
+                const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+                for (int i = 0; i < C::kAcc / 2; ++i) acc[i] = ptx::f2_pack(nan, nan);
+            }
+            if (csplit > 1) {  // the CTA's one tile: its sums to the ring (every step is consumed)
+                float *part = reinterpret_cast<float *>(smem);
+#pragma unroll
+                for (int i = 0; i < C::kAcc / 2; ++i) {
+                    if (2 * i < per) {
+                        float v0, v1;
+                        ptx::f2_unpack(acc[i], v0, v1);
+                        part[(row_off + 2 * i) * kM + col] = v0;
+                        part[(row_off + 2 * i + 1) * kM + col] = v1;
+                    }
+                }
+                break;
+            }
+            // ---- epilogue: this thread's column, its rows ----
+            const int row0 = p.rt * RT + row_off, nrows = min(per, a.rows - row0);
+            const bool up = a.gated && (col & 8);
+            const long long n = a.gated ? (long long)p.nt * (kM / 2) + (col >> 4) * 8 + (col & 7) : (long long)p.nt * kM + col;
+            const bool write = n < a.n;
+            const __half *bp = static_cast<const __half *>(up ? a.bias2 : a.bias);
+            const float bias = bp && write ? __half2float(bp[n]) : 0.f;
+            __half *y = static_cast<__half *>(a.y) + (long long)row0 * a.y_stride + n;
+            const __half *res = static_cast<const __half *>(a.residual) + (long long)row0 * a.residual_stride + n;
+#pragma unroll
+            for (int i = 0; i < C::kAcc / 2; ++i) {
+                if (2 * i < nrows) {
+                    float v0, v1;
+                    ptx::f2_unpack(acc[i], v0, v1);
+                    v0 += bias;
+                    v1 += bias;
+                    if (a.gated) {
+                        // of each pair of rows the gate's lane finishes the first, the other's the second
+                        const float got = __shfl_xor_sync(0xffffffffu, up ? v0 : v1, 8);
+                        const float o = lin::activate(a.act, up ? got : v0) * (up ? v1 : got);
+                        const int r = 2 * i + (up ? 1 : 0);
+                        if (write && r < nrows) y[(long long)r * a.y_stride] = __float2half_rn(o);
+                    } else {
+                        v0 = lin::activate(a.act, v0);
+                        v1 = lin::activate(a.act, v1);
+                        const bool two = 2 * i + 1 < nrows;
+                        if (write) {
+                            if (a.residual) {
+                                v0 += __half2float(res[(long long)(2 * i) * a.residual_stride]);
+                                if (two) v1 += __half2float(res[(long long)(2 * i + 1) * a.residual_stride]);
+                            }
+                            y[(long long)(2 * i) * a.y_stride] = __float2half_rn(v0);
+                            if (two) y[(long long)(2 * i + 1) * a.y_stride] = __float2half_rn(v1);
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    __syncwarp();
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (warp == C::kMma) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tbase, C::kTmemCols);
+    }
+    if (csplit > 1) {
+        // ---- the parts of K, in rank order, and the epilogue ----
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        const TilePos p = tile_pos(first, ntiles, nrt);
+        const float *part = reinterpret_cast<const float *>(smem);
+        const int oc = a.gated ? kM / 2 : kM, nrows = min(RT, a.rows - p.rt * RT);
+        const __half *bias = static_cast<const __half *>(a.bias), *bias2 = static_cast<const __half *>(a.bias2);
+        ptx::griddep_wait();
+        for (int i = rank * C::kThreads + threadIdx.x; i < nrows * oc; i += csplit * C::kThreads) {
+            const int r = i / oc, c = i % oc;
+            const long long n = (long long)p.nt * oc + c, row = (long long)p.rt * RT + r;
+            if (n >= a.n) continue;
+            const int c0 = a.gated ? (c >> 3) * 16 + (c & 7) : c;
+            float v = 0.f, u = 0.f;
+            for (int k = 0; k < csplit; ++k) {
+                const float *o = cluster.map_shared_rank(part + r * kM + c0, k);
+                v += o[0];
+                if (a.gated) u += o[8];
+            }
+            if (bias) v += __half2float(bias[n]);
+            v = lin::activate(a.act, v);
+            if (a.gated) {
+                if (bias2) u += __half2float(bias2[n]);
+                v *= u;
+            } else if (a.residual) {
+                v += __half2float(static_cast<const __half *>(a.residual)[row * a.residual_stride + n]);
+            }
+            static_cast<__half *>(a.y)[row * a.y_stride + n] = __float2half_rn(v);
+        }
+        __syncwarp();
+        cluster.sync();  // no CTA leaves while another may still read its shared memory
+    }
+}
+
+template <typename C>
+cudaError_t launch_t(const LinearArgs &a, unsigned grid, cudaStream_t s) {
+    static std::atomic<unsigned long long> done{0};  // devices whose shared-memory limit is set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(done.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(linear_tc_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        if (e != cudaSuccess) return e;
+        done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    Map xmap;
+    e = encode_tensor_map_2d(&xmap, true, a.x, (unsigned long long)a.k, (unsigned long long)a.rows,
+                             (unsigned long long)a.x_stride * 2, 64, (unsigned)a.row_tile);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.csplit;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, linear_tc_kernel<C>, a, xmap);
+}
+
+// At most 14 warps of 144 registers per SM. Few rows: the weight stream asks
+// for converters; many: the sums ask for drains (96 rows a thread).
+using Small = Cfg<32, 4, 4, 2>;
+using Medium = Cfg<64, 8, 4, 1>;
+using Large = Cfg<192, 4, 8, 1>;
+
+}  // namespace
+
+cudaError_t launch_linear_tc(LinearArgs a, int num_sms, cudaStream_t s) {
+    const int nrt = (a.rows + Large::kRows - 1) / Large::kRows;
+    a.row_tile = ((a.rows + nrt - 1) / nrt + 31) / 32 * 32;
+    const long long ntiles = (lin::tiles(a.n, a.gated != 0) + 1) / 2;
+    const long long total = ntiles * ((a.rows + a.row_tile - 1) / a.row_tile);
+    const bool small = a.row_tile <= Small::kRows;
+    const long long slots = (long long)num_sms * (small ? Small::kPerSm : Large::kPerSm);
+    const int nblocks = lin::blocks(a.k);
+    a.csplit = 1;
+    while (a.csplit < 8 && total * a.csplit * 2 <= slots && nblocks / (a.csplit * 2) >= 4) a.csplit *= 2;
+    const unsigned grid = (unsigned)(a.csplit > 1 ? total * a.csplit : std::min<long long>(total, slots));
+    return small ? launch_t<Small>(a, grid, s)
+           : a.row_tile <= Medium::kRows ? launch_t<Medium>(a, grid, s)
+                                         : launch_t<Large>(a, grid, s);
+}
+
+}  // namespace tllm

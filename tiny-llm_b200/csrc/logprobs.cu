@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
             if (a.top_logprobs) a.top_logprobs[at] = bad ? nan : have ? logprob(merged[n].v) : -INFINITY;
         }
     }
+    __syncwarp();
     if (split > 1) cluster.sync();  // no CTA leaves while rank 0 may still read its shared memory
 }
 
