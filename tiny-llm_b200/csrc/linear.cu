@@ -39,7 +39,7 @@ namespace cg = cooperative_groups;
 constexpr int kConsumers = 8;                      // warps
 constexpr int kThreads = 32 * (kConsumers + 1);    // + the producer warp
 constexpr int kMaxUnit = lin::unit_bytes(32);      // 8704
-constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr long long kWait = 4000000000ll;  // cycles: about 2 s
 
 template <int RB>
 struct Cfg {
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const
             int issued = 0;
             for (int i = 0; i < count; ++i, ++issued) {
                 const int s = i % C::kNS;
-                if (i >= C::kNS && !ptx::mbar_wait_bounded(empty_u + 8 * s, (uint32_t)((i / C::kNS - 1) & 1), kWaitNs)) {
+                if (i >= C::kNS && !ptx::mbar_wait_cycles(empty_u + 8 * s, (uint32_t)((i / C::kNS - 1) & 1), kWait)) {
                     s_failed = 1;
                     break;
                 }
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const
             }
             if (issued < count)  // gave up: the copies in flight land (or a bounded wait passes) before the CTA goes on
                 for (int i = max(0, issued - C::kNS); i < issued; ++i)
-                    ptx::mbar_wait_bounded(full_u + 8 * (i % C::kNS), (uint32_t)((i / C::kNS) & 1), kWaitNs);
+                    ptx::mbar_wait_cycles(full_u + 8 * (i % C::kNS), (uint32_t)((i / C::kNS) & 1), kWait);
         }
         __syncwarp();
     } else {
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const
         bool ok = true;
         for (int i = warp; i < count; i += kConsumers) {
             const int s = i % C::kNS;
-            ok = __all_sync(0xffffffffu, ptx::mbar_wait_bounded(full_u + 8 * s, (uint32_t)((i / C::kNS) & 1), kWaitNs));
+            ok = __all_sync(0xffffffffu, ptx::mbar_wait_cycles(full_u + 8 * s, (uint32_t)((i / C::kNS) & 1), kWait));
             if (!ok) break;
             const uint8_t *st = smem + s * C::kStage;
             const uint8_t *wst = st + 2 * C::kXHalf;

@@ -46,7 +46,9 @@ constexpr int kM = 128;            // packed columns of a tile
 constexpr int kStepK = 64;         // rows of K per ring stage
 constexpr int kNA = 4;             // A operand stages in TMEM (32 columns each)
 constexpr int kMaxStages = 12;
-constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr int kOutRows = 16;       // rows a drain warp writes at a time
+constexpr int kOutPitch = 36;      // floats of such a row: 32 columns, padded to 16 bytes and other banks
+constexpr long long kWait = 4000000000ll;  // cycles: about 2 s
 
 struct alignas(64) Map {  // a tensor map, opaque here
     unsigned char bytes[128];
@@ -62,9 +64,10 @@ struct Cfg {
     static constexpr int kThreads = 32 * (kDW + kCW + 2);
     static constexpr int kAcc = kRows / kDrainSets;  // rows per drain thread
     static constexpr uint32_t kTmemCols = 2 * kRows + kNA * 32 <= 128 ? 128 : 2 * kRows + kNA * 32 <= 256 ? 256 : 512;
-    static constexpr int kRing = (kPerSm == 2 ? 100 : 196) * 1024;
+    static constexpr int kRing = (kPerSm == 2 ? 96 : 192) * 1024;
+    static constexpr int kOut = kDW * kOutRows * kOutPitch * 4;  // the drain warps' rows on their way out
     static constexpr int kBars = (2 * kMaxStages + 2 * kNA + 5) * 8;
-    static constexpr int kSmem = 1024 + kRing + kBars + 16;
+    static constexpr int kSmem = 1024 + kRing + kOut + kBars + 16;
     static_assert(kAcc % 16 == 0 && kPerSm * kTmemCols <= 512, "tile");
 };
 
@@ -94,12 +97,97 @@ __device__ __forceinline__ TilePos tile_pos(int t, int ntiles, int nrt) {
     return {band * 16 + left % width, left / width};
 }
 
-template <typename C>
+// A ring position: the stage and the parity of its current round.
+struct Ring {
+    int s = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void advance(int by, int size) {
+        s += by;
+        if (s >= size) {
+            s -= size;
+            parity ^= 1u;
+        }
+    }
+};
+
+// One drain warp's [16 rows][32 packed columns] of sums, in shared memory, to
+// the output: lane = (row, half of the columns). A function of its own,
+// called for every 16 rows: inlined into the unrolled loop over a thread's
+// rows its activations alone outgrow the instruction cache (94,000 cycles a
+// tile against a few thousand).
+__device__ __noinline__ void write_rows(const LinearArgs &a, float *st, int lane, long long row0, int nrows,
+                                        long long packed0) {
+    const int r = lane >> 1, h = lane & 1;
+    if (r < nrows) {
+        float *v = st + r * kOutPitch + h * 16;
+        uint32_t *out = reinterpret_cast<uint32_t *>(v);  // pairs of outputs, over sums already read
+        const int width = a.gated ? 8 : 16;                // outputs of the lane
+        const long long n0 = (a.gated ? packed0 / 2 : packed0) + h * width;
+        const int valid = (int)min((long long)width, a.n - n0);
+        if (valid > 0) {
+            const __half *bias = static_cast<const __half *>(a.bias), *bias2 = static_cast<const __half *>(a.bias2);
+            const __half *res = a.residual ? static_cast<const __half *>(a.residual) + (row0 + r) * a.residual_stride + n0
+                                           : nullptr;
+            __half *y = static_cast<__half *>(a.y) + (row0 + r) * a.y_stride + n0;
+            // 16-byte accesses where the addresses allow them
+            const bool whole = valid == width;
+            const bool vec_y = whole && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+            const bool vec_r = whole && res && (reinterpret_cast<uintptr_t>(res) & 15) == 0;
+            if (vec_r && a.act == 0 && !bias && vec_y) {  // (never gated: residuals are the plain product's)
+                const uint4 q0 = *reinterpret_cast<const uint4 *>(res), q1 = *reinterpret_cast<const uint4 *>(res + 8);
+                const uint32_t q[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+                uint32_t o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 f = *reinterpret_cast<const float2 *>(v + 2 * j);
+                    const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&q[j]));
+                    o[j] = ptx::pack_half2(f.x + t.x, f.y + t.y);
+                }
+                *reinterpret_cast<uint4 *>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4 *>(y + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < width; j += 2) {
+                    float o[2];
+                    const int j1 = min(j + 1, valid - 1);  // an odd last column: its neighbour is not written
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int je = e ? j1 : min(j, valid - 1);
+                        float x = v[j + e];
+                        if (bias) x += __half2float(bias[n0 + je]);
+                        x = lin::activate(a.act, x);
+                        if (a.gated) {
+                            float u = v[8 + j + e];
+                            if (bias2) u += __half2float(bias2[n0 + je]);
+                            x *= u;
+                        } else if (res) {
+                            x += __half2float(res[je]);
+                        }
+                        o[e] = x;
+                    }
+                    if (vec_y) {
+                        out[j / 2] = ptx::pack_half2(o[0], o[1]);
+                    } else {
+                        if (j < valid) y[j] = __float2half_rn(o[0]);
+                        if (j + 1 < valid) y[j + 1] = __float2half_rn(o[1]);
+                    }
+                }
+                if (vec_y) {
+                    *reinterpret_cast<uint4 *>(y) = *reinterpret_cast<const uint4 *>(out);
+                    if (!a.gated) *reinterpret_cast<uint4 *>(y + 8) = *reinterpret_cast<const uint4 *>(out + 4);
+                }
+            }
+        }
+    }
+}
+
+template <typename C, bool G32>
 __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     linear_tc_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ Map xmap) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing);
+    float *out_rows = reinterpret_cast<float *>(smem + C::kRing);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing + C::kOut);
     const uint32_t full_u = ptx::smem_u32(bars);           // [stages] weights and activations landed
     const uint32_t empty_u = full_u + 8 * kMaxStages;      // [stages] converted and multiplied
     const uint32_t afull_u = empty_u + 8 * kMaxStages;     // [kNA] A operand in TMEM
@@ -119,9 +207,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     // this CTA's part of K, in blocks of 128 (whole scale groups), and its steps of 64
     const int b0 = (int)((long long)rank * nblocks / csplit), b1 = (int)((long long)(rank + 1) * nblocks / csplit);
     const int step0 = 2 * b0, steps = min(2 * b1, (a.k + kStepK - 1) / kStepK) - step0;
-    const int gsteps = a.group >= 64 ? a.group / 64 : 1;  // steps of a group
-    const int gper = a.group == 32 ? 2 : 1;               // groups of a step
-    const int ngroups = a.group == 32 ? 2 * steps : (steps + gsteps - 1) / gsteps;
+    const int gsteps = G32 ? 1 : a.group / 64;  // steps of a group (G32: a step is two groups)
+    const int ngroups = G32 ? 2 * steps : (steps + gsteps - 1) / gsteps;
     const int first = blockIdx.x / csplit, stride = gridDim.x / csplit;
     const int xbytes = RT * 128, stage_bytes = xbytes + 8192;
     const int NS = min(kMaxStages, C::kRing / stage_bytes) & ~1;  // even: a converter set meets every phase of its stages
@@ -150,125 +237,125 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     const uint32_t acol = 2 * C::kRows;
     ptx::griddep_launch_dependents();
 
-    if (warp >= C::kProd) {
-        if (warp == C::kProd && lane == 0) {
+    // (A wait for "empty" starts on the parity of the round before: a fresh
+    // barrier answers it at once.)
+    if (warp == C::kProd) {
+        if (lane == 0) {
             // ---- producer ----
             ptx::prefetch_tensormap(&xmap);
             ptx::griddep_wait();
             const uint64_t keep = ptx::l2_policy_evict_last();
             const uint64_t wpol = nrt > 1 ? keep : ptx::l2_policy_evict_first();  // weights: read once per row tile
             const uint8_t *packed = static_cast<const uint8_t *>(a.packed);
-            int it = 0;
+            const uint32_t ring_u = ptx::smem_u32(smem);
+            Ring r;
+            int issued = 0;
             bool ok = true;
             for (int t = first; t < total && ok; t += stride) {
                 const TilePos p = tile_pos(t, ntiles, nrt);
                 const bool both = 2 * p.nt + 1 < tiles64;
-                const uint8_t *w0 = packed + (long long)(2 * p.nt) * nblocks * unit;
+                const uint8_t *w0 = packed + ((long long)(2 * p.nt) * nblocks + b0) * unit;
                 const uint8_t *w1 = w0 + (long long)nblocks * unit;
-                for (int i = 0; i < steps; ++i, ++it) {
-                    const int s = it % NS;
-                    if (it >= NS && !ptx::mbar_wait_bounded(empty_u + 8 * s, (uint32_t)((it / NS - 1) & 1), kWaitNs)) {
+                const uint32_t bytes = (uint32_t)(xbytes + (both ? 2 : 1) * lin::kHalfBytes);
+                for (int i = 0; i < steps; ++i, r.advance(1, NS), ++issued) {
+                    if (!ptx::mbar_wait_cycles(empty_u + 8 * r.s, r.parity ^ 1u, kWait)) {
                         ok = false;
                         break;
                     }
-                    const int step = step0 + i;
-                    const long long off = (long long)(step >> 1) * unit + (step & 1) * lin::kHalfBytes;
-                    const uint32_t dst = ptx::smem_u32(smem + s * stage_bytes), bar = full_u + 8 * s;
-                    ptx::mbar_arrive_expect_tx(bar, (uint32_t)(xbytes + (both ? 2 : 1) * lin::kHalfBytes));
-                    ptx::bulk_load(dst + xbytes, w0 + off, lin::kHalfBytes, bar, wpol);
-                    if (both) ptx::bulk_load(dst + xbytes + lin::kHalfBytes, w1 + off, lin::kHalfBytes, bar, wpol);
-                    ptx::tma_load_2d(dst, &xmap, bar, step * kStepK, p.rt * RT, keep);
+                    const uint32_t dst = ring_u + (uint32_t)(r.s * stage_bytes), bar = full_u + 8 * r.s;
+                    ptx::mbar_arrive_expect_tx(bar, bytes);
+                    ptx::bulk_load(dst + xbytes, w0, lin::kHalfBytes, bar, wpol);
+                    if (both) ptx::bulk_load(dst + xbytes + lin::kHalfBytes, w1, lin::kHalfBytes, bar, wpol);
+                    ptx::tma_load_2d(dst, &xmap, bar, (step0 + i) * kStepK, p.rt * RT, keep);
+                    const int next = i & 1 ? unit - lin::kHalfBytes : lin::kHalfBytes;  // the block's other half, the next block
+                    w0 += next;
+                    w1 += next;
                 }
             }
-            if (!ok) {
-                // the copies in flight land (or a bounded wait passes) before the CTA goes on
-                for (int i = max(0, it - NS); i < it; ++i)
-                    ptx::mbar_wait_bounded(full_u + 8 * (i % NS), (uint32_t)((i / NS) & 1), kWaitNs);
-            }
-        } else if (warp == C::kMma && lane == 0) {
+            if (!ok)  // the copies in flight land (or a bounded wait passes) before the CTA goes on
+                for (int i = max(0, issued - NS); i < issued; ++i)
+                    ptx::mbar_wait_cycles(full_u + 8 * (i % NS), (uint32_t)((i / NS) & 1), kWait);
+        }
+    } else if (warp == C::kMma) {
+        if (lane == 0) {
             // ---- UMMA issue ----
             const uint32_t idesc = (1u << 4) | ((uint32_t)(RT >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
-            const uint32_t ring_u = ptx::smem_u32(smem);
-            int it = 0, gi = 0;  // steps and groups over all tiles
+            const uint64_t desc0 = ptx::umma_desc_sw128(ptx::smem_u32(smem), 16, 1024);
+            Ring r, aa, dd;  // ring stage, A stage, accumulator
             bool ok = true;
             for (int t = first; t < total && ok; t += stride) {
                 int in_group = 0;  // steps of the group done
-                for (int i = 0; i < steps; ++i, ++it) {
-                    const int s = it % NS, j = it % kNA;
-                    if (in_group == 0 && gi >= 2 &&
-                        !ptx::mbar_wait_bounded(dempty_u + 8 * (gi & 1), (uint32_t)((gi / 2 - 1) & 1), kWaitNs))
-                        ok = false;
-                    ok = ok && ptx::mbar_wait_bounded(full_u + 8 * s, (uint32_t)((it / NS) & 1), kWaitNs) &&
-                         ptx::mbar_wait_bounded(afull_u + 8 * j, (uint32_t)((it / kNA) & 1), kWaitNs);
+                for (int i = 0; i < steps; ++i) {
+                    if (in_group == 0) ok = ptx::mbar_wait_cycles(dempty_u + 8 * dd.s, dd.parity ^ 1u, kWait);
+                    ok = ok && ptx::mbar_wait_cycles(full_u + 8 * r.s, r.parity, kWait) &&
+                         ptx::mbar_wait_cycles(afull_u + 8 * aa.s, aa.parity, kWait);
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
-                    const uint32_t xa = ring_u + (uint32_t)(s * stage_bytes);
-                    const uint32_t at = tbase + acol + (uint32_t)(j * 32);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        if (ks == 2 && gper == 2) {  // the step's second group
-                            ptx::umma_commit(dfull_u + 8 * (gi & 1));
-                            ++gi;
-                            if (gi >= 2 &&
-                                !ptx::mbar_wait_bounded(dempty_u + 8 * (gi & 1), (uint32_t)((gi / 2 - 1) & 1), kWaitNs)) {
-                                ok = false;
-                                break;
-                            }
-                            ptx::tc_fence_after_sync();
-                        }
-                        const bool fresh = ks == 0 ? in_group == 0 : (ks == 2 && gper == 2);
-                        ptx::umma_f16_ta(tbase + (uint32_t)((gi & 1) * C::kRows), at + (uint32_t)(8 * ks),
-                                         ptx::umma_desc_sw128(xa + ks * 32, 16, 1024), idesc, fresh ? 0u : 1u);
+                    const uint64_t bd = desc0 + (uint64_t)((uint32_t)(r.s * stage_bytes) >> 4);  // addresses in 16 bytes
+                    const uint32_t at = tbase + acol + (uint32_t)(aa.s * 32);
+                    uint32_t dt = tbase + (uint32_t)(dd.s * C::kRows);
+                    ptx::umma_f16_ta(dt, at, bd, idesc, in_group == 0 ? 0u : 1u);
+                    ptx::umma_f16_ta(dt, at + 8, bd + 2, idesc, 1u);
+                    if constexpr (G32) {  // the step's second group
+                        ptx::umma_commit(dfull_u + 8 * dd.s);
+                        dd.advance(1, 2);
+                        ok = ptx::mbar_wait_cycles(dempty_u + 8 * dd.s, dd.parity ^ 1u, kWait);
+                        if (!ok) break;
+                        ptx::tc_fence_after_sync();
+                        dt = tbase + (uint32_t)(dd.s * C::kRows);
                     }
-                    if (!ok) break;
-                    ptx::umma_commit(aempty_u + 8 * j);
-                    ptx::umma_commit(empty_u + 8 * s);
+                    ptx::umma_f16_ta(dt, at + 16, bd + 4, idesc, G32 ? 0u : 1u);
+                    ptx::umma_f16_ta(dt, at + 24, bd + 6, idesc, 1u);
+                    ptx::umma_commit(aempty_u + 8 * aa.s);
+                    ptx::umma_commit(empty_u + 8 * r.s);
                     if (++in_group == gsteps || i + 1 == steps) {
-                        ptx::umma_commit(dfull_u + 8 * (gi & 1));
-                        ++gi;
+                        ptx::umma_commit(dfull_u + 8 * dd.s);
+                        dd.advance(1, 2);
                         in_group = 0;
                     }
+                    r.advance(1, NS);
+                    aa.advance(1, kNA);
                 }
             }
             // every UMMA issued is complete before TMEM is freed
             ptx::umma_commit(done_u);
-            ptx::mbar_wait_bounded(done_u, 0u, kWaitNs);
+            ptx::mbar_wait_cycles(done_u, 0u, kWait);
         }
     } else if (warp >= C::kDW) {
         // ---- converters: set c takes steps c, c + kConvSets, ... ----
         const int set = (warp - C::kDW) >> 2, q = warp & 3;
         const int n64 = (q & 1) * 32 + lane;
-        const uint32_t roff = (uint32_t)(xbytes + (q >> 1) * lin::kHalfBytes);
+        const uint8_t *raw0 = smem + xbytes + (q >> 1) * lin::kHalfBytes;
+        const uint32_t at0 = tbase + ((uint32_t)(32 * q) << 16) + acol;
         const int my_tiles = first < total ? (total - first + stride - 1) / stride : 0;
         const int all = my_tiles * steps;
-        bool ok = true;
+        Ring r, aa;
+        r.s = aa.s = set;
         for (int it = set; it < all; it += C::kConvSets) {
-            const int s = it % NS, j = it % kNA;
-            ok = ptx::mbar_wait_bounded(full_u + 8 * s, (uint32_t)((it / NS) & 1), kWaitNs);
-            ok = ok && (it < kNA || ptx::mbar_wait_bounded(aempty_u + 8 * j, (uint32_t)((it / kNA - 1) & 1), kWaitNs));
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
-            }
+            const bool ok = ptx::mbar_wait_cycles(full_u + 8 * r.s, r.parity, kWait) &&
+                            ptx::mbar_wait_cycles(aempty_u + 8 * aa.s, aa.parity ^ 1u, kWait);
+            if (!__all_sync(0xffffffffu, ok)) break;
             ptx::tc_fence_after_sync();
-            const uint8_t *raw = smem + s * stage_bytes + roff;
-            uint32_t r[32];
+            const uint8_t *raw = raw0 + r.s * stage_bytes;
+            uint32_t f[32];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const uint4 v = *reinterpret_cast<const uint4 *>(raw + c * 1024 + ((n64 ^ (2 * c)) << 4));
-                lin::to_h4(v.x, r[4 * c], r[4 * c + 1]);
-                lin::to_h4(v.y, r[4 * c + 2], r[4 * c + 3]);
-                lin::to_h4(v.z, r[16 + 4 * c], r[16 + 4 * c + 1]);
-                lin::to_h4(v.w, r[16 + 4 * c + 2], r[16 + 4 * c + 3]);
+                lin::to_h4(v.x, f[4 * c], f[4 * c + 1]);
+                lin::to_h4(v.y, f[4 * c + 2], f[4 * c + 3]);
+                lin::to_h4(v.z, f[16 + 4 * c], f[16 + 4 * c + 1]);
+                lin::to_h4(v.w, f[16 + 4 * c + 2], f[16 + 4 * c + 3]);
             }
-            ptx::tmem_st32(tbase + ((uint32_t)(32 * q) << 16) + acol + (uint32_t)(j * 32), r);
+            ptx::tmem_st32(at0 + (uint32_t)(aa.s * 32), f);
             ptx::tmem_wait_st();
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
-                ptx::mbar_arrive(afull_u + 8 * j);
-                ptx::mbar_arrive(empty_u + 8 * s);
+                ptx::mbar_arrive(afull_u + 8 * aa.s);
+                ptx::mbar_arrive(empty_u + 8 * r.s);
             }
+            r.advance(C::kConvSets, NS);
+            aa.advance(C::kConvSets, kNA);
         }
     } else {
         // ---- drains ----
@@ -277,50 +364,55 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         const int per = RT / C::kDrainSets;         // rows of a drain thread, a multiple of 16
         const int row_off = set * per;
         const uint32_t tlane = tbase + ((uint32_t)(32 * q) << 16) + (uint32_t)row_off;
-        int gi = 0;
+        float *st = out_rows + warp * kOutRows * kOutPitch;
+        Ring dd;
         bool ok = true;
         ptx::griddep_wait();
         for (int t = first; t < total; t += stride) {
             const TilePos p = tile_pos(t, ntiles, nrt);
             const int t64 = 2 * p.nt + (q >> 1);
-            const bool real = t64 < tiles64;
-            // scales of this column, one per group
-            const uint8_t *sbase = static_cast<const uint8_t *>(a.packed) + ((long long)(real ? t64 : 0) * nblocks + b0) * unit +
-                                   2 * lin::kHalfBytes + (col & 63) * 2;
-            const int gshift = a.group == 32 ? 2 : a.group == 64 ? 1 : 0;  // log2 of the groups of a block
-            auto scale_of = [&](int g) -> float {
-                const uint8_t *sp = sbase + (long long)(g >> gshift) * unit + (g & ((1 << gshift) - 1)) * (lin::kTileN * 2);
-                return __half2float(__ushort_as_half(__ldg(reinterpret_cast<const unsigned short *>(sp))));
+            // this column's scales, one per group (a tile's missing second half: any)
+            const int gsub = lin::kBlockK / a.group;  // groups of a block
+            const uint8_t *sp = static_cast<const uint8_t *>(a.packed) +
+                                ((long long)(t64 < tiles64 ? t64 : 0) * nblocks + b0) * unit + 2 * lin::kHalfBytes +
+                                (col & 63) * 2;
+            int sub = 0;
+            auto next_scale = [&]() -> float {
+                const float v = __half2float(__ushort_as_half(__ldg(reinterpret_cast<const unsigned short *>(sp))));
+                if (++sub == gsub) {
+                    sub = 0;
+                    sp += unit - (gsub - 1) * (lin::kTileN * 2);
+                } else {
+                    sp += lin::kTileN * 2;
+                }
+                return v;
             };
             uint64_t acc[C::kAcc / 2];  // pairs of rows
 #pragma unroll
             for (int i = 0; i < C::kAcc / 2; ++i) acc[i] = 0ull;
-            float sc = scale_of(0);
-            for (int g = 0; g < ngroups; ++g, ++gi) {
+            float sc = next_scale();
+            for (int g = 0; g < ngroups; ++g, dd.advance(1, 2)) {
                 const uint64_t s2 = ptx::f2_pack(sc, sc);
-                if (g + 1 < ngroups) sc = scale_of(g + 1);
-                if (ok)
-                    ok = __all_sync(0xffffffffu,
-                                    ptx::mbar_wait_bounded(dfull_u + 8 * (gi & 1), (uint32_t)((gi / 2) & 1), kWaitNs));
-                if (ok) {
-                    ptx::tc_fence_after_sync();
+                if (g + 1 < ngroups) sc = next_scale();
+                ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait_cycles(dfull_u + 8 * dd.s, dd.parity, kWait));
+                if (!ok) continue;
+                ptx::tc_fence_after_sync();
 #pragma unroll
-                    for (int c = 0; c < C::kAcc / 16; ++c) {
-                        if (c * 16 < per) {
-                            uint32_t v[16];
-                            tmem_ld16(tlane + (uint32_t)((gi & 1) * C::kRows + c * 16), v);
-                            tmem_wait_ld16(v);
+                for (int c = 0; c < C::kAcc / 16; ++c) {
+                    if (c * 16 < per) {
+                        uint32_t v[16];
+                        tmem_ld16(tlane + (uint32_t)(dd.s * C::kRows + c * 16), v);
+                        tmem_wait_ld16(v);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                acc[c * 8 + i] = ptx::f2_fma(
-                                    ptx::f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), s2,
-                                    acc[c * 8 + i]);
-                        }
+                        for (int i = 0; i < 8; ++i)
+                            acc[c * 8 + i] =
+                                ptx::f2_fma(ptx::f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), s2,
+                                            acc[c * 8 + i]);
                     }
-                    ptx::tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(dempty_u + 8 * (gi & 1));
                 }
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(dempty_u + 8 * dd.s);
             }
             if (!ok) {
                 const float nan = __int_as_float(0x7fffffff);
@@ -340,41 +432,22 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 }
                 break;
             }
-            // ---- epilogue: this thread's column, its rows ----
-            const int row0 = p.rt * RT + row_off, nrows = min(per, a.rows - row0);
-            const bool up = a.gated && (col & 8);
-            const long long n = a.gated ? (long long)p.nt * (kM / 2) + (col >> 4) * 8 + (col & 7) : (long long)p.nt * kM + col;
-            const bool write = n < a.n;
-            const __half *bp = static_cast<const __half *>(up ? a.bias2 : a.bias);
-            const float bias = bp && write ? __half2float(bp[n]) : 0.f;
-            __half *y = static_cast<__half *>(a.y) + (long long)row0 * a.y_stride + n;
-            const __half *res = static_cast<const __half *>(a.residual) + (long long)row0 * a.residual_stride + n;
+            // ---- epilogue: 16 rows at a time through shared memory ----
+            const long long row0 = (long long)p.rt * RT + row_off;
+            const int nrows = (int)min((long long)per, a.rows - row0);
 #pragma unroll
-            for (int i = 0; i < C::kAcc / 2; ++i) {
-                if (2 * i < nrows) {
-                    float v0, v1;
-                    ptx::f2_unpack(acc[i], v0, v1);
-                    v0 += bias;
-                    v1 += bias;
-                    if (a.gated) {
-                        // of each pair of rows the gate's lane finishes the first, the other's the second
-                        const float got = __shfl_xor_sync(0xffffffffu, up ? v0 : v1, 8);
-                        const float o = lin::activate(a.act, up ? got : v0) * (up ? v1 : got);
-                        const int r = 2 * i + (up ? 1 : 0);
-                        if (write && r < nrows) y[(long long)r * a.y_stride] = __float2half_rn(o);
-                    } else {
-                        v0 = lin::activate(a.act, v0);
-                        v1 = lin::activate(a.act, v1);
-                        const bool two = 2 * i + 1 < nrows;
-                        if (write) {
-                            if (a.residual) {
-                                v0 += __half2float(res[(long long)(2 * i) * a.residual_stride]);
-                                if (two) v1 += __half2float(res[(long long)(2 * i + 1) * a.residual_stride]);
-                            }
-                            y[(long long)(2 * i) * a.y_stride] = __float2half_rn(v0);
-                            if (two) y[(long long)(2 * i + 1) * a.y_stride] = __float2half_rn(v1);
-                        }
+            for (int c = 0; c < C::kAcc / 16; ++c) {
+                if (c * 16 < nrows) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float v0, v1;
+                        ptx::f2_unpack(acc[c * 8 + i], v0, v1);
+                        st[(2 * i) * kOutPitch + lane] = v0;
+                        st[(2 * i + 1) * kOutPitch + lane] = v1;
                     }
+                    __syncwarp();
+                    write_rows(a, st, lane, row0 + c * 16, min(16, nrows - c * 16), (long long)p.nt * kM + 32 * q);
+                    __syncwarp();
                 }
             }
         }
@@ -390,6 +463,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     if (csplit > 1) {
         // ---- the parts of K, in rank order, and the epilogue ----
         cg::cluster_group cluster = cg::this_cluster();
+        __syncwarp();
         cluster.sync();
         const TilePos p = tile_pos(first, ntiles, nrt);
         const float *part = reinterpret_cast<const float *>(smem);
@@ -422,15 +496,15 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     }
 }
 
-template <typename C>
-cudaError_t launch_t(const LinearArgs &a, unsigned grid, cudaStream_t s) {
+template <typename C, bool G32>
+cudaError_t launch_g(const LinearArgs &a, unsigned grid, cudaStream_t s) {
     static std::atomic<unsigned long long> done{0};  // devices whose shared-memory limit is set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(linear_tc_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        e = cudaFuncSetAttribute(linear_tc_kernel<C, G32>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
         if (e != cudaSuccess) return e;
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
@@ -451,7 +525,12 @@ cudaError_t launch_t(const LinearArgs &a, unsigned grid, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, linear_tc_kernel<C>, a, xmap);
+    return cudaLaunchKernelEx(&cfg, linear_tc_kernel<C, G32>, a, xmap);
+}
+
+template <typename C>
+cudaError_t launch_t(const LinearArgs &a, unsigned grid, cudaStream_t s) {
+    return a.group == 32 ? launch_g<C, true>(a, grid, s) : launch_g<C, false>(a, grid, s);
 }
 
 // At most 14 warps of 144 registers per SM. Few rows: the weight stream asks

@@ -168,6 +168,19 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
     }
 }
 
+// The same, bounded in SM clock cycles: reading the clock takes a few cycles
+// where %globaltimer takes about a microsecond, which a pipeline whose stages
+// wait for one another pays at every wait that does not succeed at once.
+__device__ __forceinline__ bool mbar_wait_cycles(uint32_t bar, uint32_t parity, long long limit) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    for (;;) {
+        for (int i = 0; i < 16; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (clock64() - t0 > limit) return false;
+    }
+}
+
 // 3-D tiled TMA load global -> shared, completing on an mbarrier. No
 // multicast: the source is always this GPU's own pool.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, uint32_t bar, int x,
