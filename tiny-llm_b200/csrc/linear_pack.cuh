@@ -60,8 +60,10 @@ __device__ __forceinline__ float activate(int act, float v) {
     // 1 + erf(t) = erfc(-t) and (1 + tanh(t)) / 2 = 1 / (1 + exp(-2t)): no
     // cancellation where the result is small
     case 2: return 0.5f * v * erfcf(-0.70710678118654752f * v);
-    case 3: return v / (1.f + expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
-    case 4: return v / (1.f + expf(-v));
+    // (the exponential and the division by the fast forms: a few fp32 units,
+    // next to the output's 2^-11)
+    case 3: return __fdividef(v, 1.f + __expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
+    case 4: return __fdividef(v, 1.f + __expf(-v));
     default: return v;
     }
 }

@@ -4,24 +4,31 @@
 //
 // The packed weight columns are the M side of the UMMA (128 per tile: two
 // tiles of 64 of the packed layout), a tile of up to 192 batch rows the N
-// side, K in steps of 64. The int8 weights become the fp16 A operand on the
-// way, exactly and in TMEM; their scales multiply the fp32 sums of one scale
-// group, so no weight is rounded and no fp16 copy of the weights exists in
-// HBM or shared memory. Per CTA:
-//   producer    one lane: per step two 4 KB bulk copies of packed weights and
-//               one TMA tile of activations [rows][64] (128-byte swizzle,
+// side, K in steps of 128 (a block of the packed layout). The int8 weights
+// become the fp16 A operand on the way, exactly and in TMEM; their scales
+// multiply the fp32 sums of one scale group, so no weight is rounded and no
+// fp16 copy of the weights exists in HBM or shared memory. Per CTA:
+//   producer    one lane: per step two 8 KB bulk copies of packed weights and
+//               two TMA tiles of activations [rows][64] (128-byte swizzle,
 //               zeros past K and the last row) into a ring of stages;
 //   converters  thread = weight column: 64 bytes from shared memory, to 64
-//               fp16, one tcgen05.st of 32 columns: the K-major A operand;
-//   MMA         one thread: four UMMAs (K = 16) per step, A in TMEM, B in
+//               fp16, one tcgen05.st of 32 columns: the K-major A operand of
+//               half a step (four warps do both halves, eight one each);
+//   MMA         one thread: eight UMMAs (K = 16) per step, A in TMEM, B in
 //               shared memory, into one of two accumulators, changed with
 //               every scale group;
 //   drains      thread = weight column (TMEM lane): when a group is complete,
 //               acc += scale * sum for the thread's rows, in registers; after
-//               the last group the epilogue straight from them.
+//               the last group the epilogue from them.
 // So the tensor cores never wait for the scaling (the other accumulator is
-// filled meanwhile) nor for a tile's epilogue: the CTAs are persistent and
-// the next tile's groups start while the last one's is written.
+// filled meanwhile), and the CTAs are persistent: the next tile's first
+// groups run while a tile's outputs are written.
+//
+// What bounds it is the MMA thread: a wait that succeeds at once costs it
+// about 110 cycles, a commit 80, a UMMA 75 or its pipe time (rows / 2). So a
+// step is as deep as the layout's block, the stage and the A operand are
+// released by one commit, and the thread does not wait for the activations:
+// the converters waited for the same barrier before they arrived.
 //
 // Too few tiles for the SMs: a cluster's CTAs share a tile's K and add their
 // sums in distributed shared memory, in rank order. No atomics, no workspace:
@@ -43,9 +50,11 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kM = 128;            // packed columns of a tile
-constexpr int kStepK = 64;         // rows of K per ring stage
-constexpr int kNA = 4;             // A operand stages in TMEM (32 columns each)
-constexpr int kMaxStages = 12;
+constexpr int kStepK = lin::kBlockK;  // rows of K per ring stage
+constexpr int kNA = 2;             // A operand stages in TMEM
+constexpr int kACols = kStepK / 2;  // TMEM columns of one (fp16 pairs along K)
+constexpr int kRaw = 2 * 2 * lin::kHalfBytes;  // packed weights of a step
+constexpr int kMaxStages = 8;
 constexpr int kOutRows = 16;       // rows a drain warp writes at a time
 constexpr int kOutPitch = 36;      // floats of such a row: 32 columns, padded to 16 bytes and other banks
 constexpr long long kWait = 4000000000ll;  // cycles: about 2 s
@@ -63,10 +72,10 @@ struct Cfg {
     static constexpr int kProd = kDW + kCW, kMma = kProd + 1;  // warps
     static constexpr int kThreads = 32 * (kDW + kCW + 2);
     static constexpr int kAcc = kRows / kDrainSets;  // rows per drain thread
-    static constexpr uint32_t kTmemCols = 2 * kRows + kNA * 32 <= 128 ? 128 : 2 * kRows + kNA * 32 <= 256 ? 256 : 512;
+    static constexpr uint32_t kTmemCols = 2 * kRows + kNA * kACols <= 256 ? 256 : 512;
     static constexpr int kRing = (kPerSm == 2 ? 96 : 192) * 1024;
     static constexpr int kOut = kDW * kOutRows * kOutPitch * 4;  // the drain warps' rows on their way out
-    static constexpr int kBars = (2 * kMaxStages + 2 * kNA + 5) * 8;
+    static constexpr int kBars = (2 * kMaxStages + kNA + 5) * 8;
     static constexpr int kSmem = 1024 + kRing + kOut + kBars + 16;
     static_assert(kAcc % 16 == 0 && kPerSm * kTmemCols <= 512, "tile");
 };
@@ -114,74 +123,68 @@ struct Ring {
 // the output: lane = (row, half of the columns). A function of its own,
 // called for every 16 rows: inlined into the unrolled loop over a thread's
 // rows its activations alone outgrow the instruction cache (94,000 cycles a
-// tile against a few thousand).
-__device__ __noinline__ void write_rows(const LinearArgs &a, float *st, int lane, long long row0, int nrows,
-                                        long long packed0) {
+// tile against a few thousand). q0, q1: the lane's residuals where `have_res`.
+template <int ACT, bool GATED>
+__device__ __noinline__ void write_rows(const LinearArgs &a, const float *st, int lane, long long row0, int nrows,
+                                        long long packed0, bool have_res, uint4 q0, uint4 q1) {
+    constexpr int W = GATED ? 8 : 16;  // outputs of the lane
     const int r = lane >> 1, h = lane & 1;
-    if (r < nrows) {
-        float *v = st + r * kOutPitch + h * 16;
-        uint32_t *out = reinterpret_cast<uint32_t *>(v);  // pairs of outputs, over sums already read
-        const int width = a.gated ? 8 : 16;                // outputs of the lane
-        const long long n0 = (a.gated ? packed0 / 2 : packed0) + h * width;
-        const int valid = (int)min((long long)width, a.n - n0);
-        if (valid > 0) {
-            const __half *bias = static_cast<const __half *>(a.bias), *bias2 = static_cast<const __half *>(a.bias2);
-            const __half *res = a.residual ? static_cast<const __half *>(a.residual) + (row0 + r) * a.residual_stride + n0
-                                           : nullptr;
-            __half *y = static_cast<__half *>(a.y) + (row0 + r) * a.y_stride + n0;
-            // 16-byte accesses where the addresses allow them
-            const bool whole = valid == width;
-            const bool vec_y = whole && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
-            const bool vec_r = whole && res && (reinterpret_cast<uintptr_t>(res) & 15) == 0;
-            if (vec_r && a.act == 0 && !bias && vec_y) {  // (never gated: residuals are the plain product's)
-                const uint4 q0 = *reinterpret_cast<const uint4 *>(res), q1 = *reinterpret_cast<const uint4 *>(res + 8);
-                const uint32_t q[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-                uint32_t o[8];
+    const long long n0 = (GATED ? packed0 / 2 : packed0) + h * W;
+    const int valid = (int)min((long long)W, a.n - n0);
+    if (r >= nrows || valid <= 0) return;
+    const float *v = st + r * kOutPitch + h * 16;
+    const __half *bias = static_cast<const __half *>(a.bias), *bias2 = static_cast<const __half *>(a.bias2);
+    const __half *res =
+        a.residual ? static_cast<const __half *>(a.residual) + (row0 + r) * a.residual_stride + n0 : nullptr;
+    __half *y = static_cast<__half *>(a.y) + (row0 + r) * a.y_stride + n0;
+    const uint32_t q[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+    uint32_t o[W / 2];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float2 f = *reinterpret_cast<const float2 *>(v + 2 * j);
-                    const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&q[j]));
-                    o[j] = ptx::pack_half2(f.x + t.x, f.y + t.y);
-                }
-                *reinterpret_cast<uint4 *>(y) = make_uint4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<uint4 *>(y + 8) = make_uint4(o[4], o[5], o[6], o[7]);
-            } else {
-#pragma unroll 1
-                for (int j = 0; j < width; j += 2) {
-                    float o[2];
-                    const int j1 = min(j + 1, valid - 1);  // an odd last column: its neighbour is not written
+    for (int j = 0; j < W; j += 2) {
+        float f[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int je = e ? j1 : min(j, valid - 1);
-                        float x = v[j + e];
-                        if (bias) x += __half2float(bias[n0 + je]);
-                        x = lin::activate(a.act, x);
-                        if (a.gated) {
-                            float u = v[8 + j + e];
-                            if (bias2) u += __half2float(bias2[n0 + je]);
-                            x *= u;
-                        } else if (res) {
-                            x += __half2float(res[je]);
-                        }
-                        o[e] = x;
-                    }
-                    if (vec_y) {
-                        out[j / 2] = ptx::pack_half2(o[0], o[1]);
-                    } else {
-                        if (j < valid) y[j] = __float2half_rn(o[0]);
-                        if (j + 1 < valid) y[j + 1] = __float2half_rn(o[1]);
-                    }
-                }
-                if (vec_y) {
-                    *reinterpret_cast<uint4 *>(y) = *reinterpret_cast<const uint4 *>(out);
-                    if (!a.gated) *reinterpret_cast<uint4 *>(y + 8) = *reinterpret_cast<const uint4 *>(out + 4);
-                }
+        for (int e = 0; e < 2; ++e) {
+            const int at = min(j + e, valid - 1);  // (outputs past the last column are not written)
+            float x = v[j + e];
+            if (bias) x += __half2float(bias[n0 + at]);
+            x = lin::activate(ACT, x);
+            if constexpr (GATED) {
+                float u = v[8 + j + e];
+                if (bias2) u += __half2float(bias2[n0 + at]);
+                x *= u;
+            } else if (have_res) {
+                x += __half2float(__ushort_as_half((unsigned short)(q[j / 2] >> (16 * e))));
+            } else if (res) {
+                x += __half2float(res[at]);
             }
+            f[e] = x;
         }
+        o[j / 2] = ptx::pack_half2(f[0], f[1]);
+    }
+    if (valid == W && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+        *reinterpret_cast<uint4 *>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+        if constexpr (!GATED) *reinterpret_cast<uint4 *>(y + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (j < valid) y[j] = __ushort_as_half((unsigned short)(o[j / 2] >> (16 * (j & 1))));
     }
 }
 
-template <typename C, bool G32>
+template <bool GATED>
+__device__ __forceinline__ void write_rows_act(const LinearArgs &a, const float *st, int lane, long long row0, int nrows,
+                                               long long packed0, bool have_res, uint4 q0, uint4 q1) {
+    switch (a.act) {
+    case 1: return write_rows<1, GATED>(a, st, lane, row0, nrows, packed0, have_res, q0, q1);
+    case 2: return write_rows<2, GATED>(a, st, lane, row0, nrows, packed0, have_res, q0, q1);
+    case 3: return write_rows<3, GATED>(a, st, lane, row0, nrows, packed0, have_res, q0, q1);
+    case 4: return write_rows<4, GATED>(a, st, lane, row0, nrows, packed0, have_res, q0, q1);
+    default: return write_rows<0, GATED>(a, st, lane, row0, nrows, packed0, have_res, q0, q1);
+    }
+}
+
+// GPS: scale groups of a step (128 / group).
+template <typename C, int GPS>
 __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     linear_tc_kernel(const __grid_constant__ LinearArgs a, const __grid_constant__ Map xmap) {
     extern __shared__ uint8_t smem_raw[];
@@ -189,10 +192,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     float *out_rows = reinterpret_cast<float *>(smem + C::kRing);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing + C::kOut);
     const uint32_t full_u = ptx::smem_u32(bars);           // [stages] weights and activations landed
-    const uint32_t empty_u = full_u + 8 * kMaxStages;      // [stages] converted and multiplied
+    const uint32_t empty_u = full_u + 8 * kMaxStages;      // [stages] multiplied: the stage and its A operand are free
     const uint32_t afull_u = empty_u + 8 * kMaxStages;     // [kNA] A operand in TMEM
-    const uint32_t aempty_u = afull_u + 8 * kNA;           // [kNA] A operand multiplied
-    const uint32_t dfull_u = aempty_u + 8 * kNA;           // [2] a group's sums complete
+    const uint32_t dfull_u = afull_u + 8 * kNA;            // [2] a group's sums complete
     const uint32_t dempty_u = dfull_u + 16;                // [2] ... and drained
     const uint32_t done_u = dempty_u + 16;                 // every UMMA complete
     __shared__ uint32_t s_tmem;
@@ -204,24 +206,19 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     const int ntiles = (tiles64 + 1) / 2, total = ntiles * nrt;
     const int csplit = a.csplit, rank = blockIdx.x % csplit;
     const int nblocks = lin::blocks(a.k), unit = lin::unit_bytes(a.group);
-    // this CTA's part of K, in blocks of 128 (whole scale groups), and its steps of 64
+    // this CTA's part of K, in blocks of 128: its steps
     const int b0 = (int)((long long)rank * nblocks / csplit), b1 = (int)((long long)(rank + 1) * nblocks / csplit);
-    const int step0 = 2 * b0, steps = min(2 * b1, (a.k + kStepK - 1) / kStepK) - step0;
-    const int gsteps = G32 ? 1 : a.group / 64;  // steps of a group (G32: a step is two groups)
-    const int ngroups = G32 ? 2 * steps : (steps + gsteps - 1) / gsteps;
+    const int steps = b1 - b0;
     const int first = blockIdx.x / csplit, stride = gridDim.x / csplit;
-    const int xbytes = RT * 128, stage_bytes = xbytes + 8192;
-    const int NS = min(kMaxStages, C::kRing / stage_bytes) & ~1;  // even: a converter set meets every phase of its stages
+    const int xhalf = RT * 128, stage_bytes = 2 * xhalf + kRaw;
+    const int NS = min(kMaxStages, C::kRing / stage_bytes);  // > kNA: a converter meets every phase it waits for
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMaxStages; ++s) {
             ptx::mbar_init(full_u + 8 * s, 1);
-            ptx::mbar_init(empty_u + 8 * s, 4 + 1);  // a converter set's warps and the MMA's commit
+            ptx::mbar_init(empty_u + 8 * s, 1);
         }
-        for (int s = 0; s < kNA; ++s) {
-            ptx::mbar_init(afull_u + 8 * s, 4);
-            ptx::mbar_init(aempty_u + 8 * s, 1);
-        }
+        for (int s = 0; s < kNA; ++s) ptx::mbar_init(afull_u + 8 * s, C::kCW);
         for (int s = 0; s < 2; ++s) {
             ptx::mbar_init(dfull_u + 8 * s, 1);
             ptx::mbar_init(dempty_u + 8 * s, C::kDW);
@@ -256,7 +253,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 const bool both = 2 * p.nt + 1 < tiles64;
                 const uint8_t *w0 = packed + ((long long)(2 * p.nt) * nblocks + b0) * unit;
                 const uint8_t *w1 = w0 + (long long)nblocks * unit;
-                const uint32_t bytes = (uint32_t)(xbytes + (both ? 2 : 1) * lin::kHalfBytes);
+                const uint32_t bytes = (uint32_t)(2 * xhalf + (both ? 2 : 1) * 2 * lin::kHalfBytes);
                 for (int i = 0; i < steps; ++i, r.advance(1, NS), ++issued) {
                     if (!ptx::mbar_wait_cycles(empty_u + 8 * r.s, r.parity ^ 1u, kWait)) {
                         ok = false;
@@ -264,12 +261,13 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     }
                     const uint32_t dst = ring_u + (uint32_t)(r.s * stage_bytes), bar = full_u + 8 * r.s;
                     ptx::mbar_arrive_expect_tx(bar, bytes);
-                    ptx::bulk_load(dst + xbytes, w0, lin::kHalfBytes, bar, wpol);
-                    if (both) ptx::bulk_load(dst + xbytes + lin::kHalfBytes, w1, lin::kHalfBytes, bar, wpol);
-                    ptx::tma_load_2d(dst, &xmap, bar, (step0 + i) * kStepK, p.rt * RT, keep);
-                    const int next = i & 1 ? unit - lin::kHalfBytes : lin::kHalfBytes;  // the block's other half, the next block
-                    w0 += next;
-                    w1 += next;
+                    ptx::bulk_load(dst + 2 * xhalf, w0, 2 * lin::kHalfBytes, bar, wpol);
+                    if (both) ptx::bulk_load(dst + 2 * xhalf + 2 * lin::kHalfBytes, w1, 2 * lin::kHalfBytes, bar, wpol);
+                    const int k0 = (b0 + i) * kStepK;  // (a half past K lies wholly out of bounds: zeros)
+                    ptx::tma_load_2d(dst, &xmap, bar, k0, p.rt * RT, keep);
+                    ptx::tma_load_2d(dst + xhalf, &xmap, bar, k0 + 64, p.rt * RT, keep);
+                    w0 += unit;
+                    w1 += unit;
                 }
             }
             if (!ok)  // the copies in flight land (or a bounded wait passes) before the CTA goes on
@@ -283,79 +281,73 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             const uint64_t desc0 = ptx::umma_desc_sw128(ptx::smem_u32(smem), 16, 1024);
             Ring r, aa, dd;  // ring stage, A stage, accumulator
             bool ok = true;
-            for (int t = first; t < total && ok; t += stride) {
-                int in_group = 0;  // steps of the group done
-                for (int i = 0; i < steps; ++i) {
-                    if (in_group == 0) ok = ptx::mbar_wait_cycles(dempty_u + 8 * dd.s, dd.parity ^ 1u, kWait);
-                    ok = ok && ptx::mbar_wait_cycles(full_u + 8 * r.s, r.parity, kWait) &&
-                         ptx::mbar_wait_cycles(afull_u + 8 * aa.s, aa.parity, kWait);
-                    if (!ok) break;
-                    ptx::tc_fence_after_sync();
-                    const uint64_t bd = desc0 + (uint64_t)((uint32_t)(r.s * stage_bytes) >> 4);  // addresses in 16 bytes
-                    const uint32_t at = tbase + acol + (uint32_t)(aa.s * 32);
-                    uint32_t dt = tbase + (uint32_t)(dd.s * C::kRows);
-                    ptx::umma_f16_ta(dt, at, bd, idesc, in_group == 0 ? 0u : 1u);
-                    ptx::umma_f16_ta(dt, at + 8, bd + 2, idesc, 1u);
-                    if constexpr (G32) {  // the step's second group
-                        ptx::umma_commit(dfull_u + 8 * dd.s);
-                        dd.advance(1, 2);
-                        ok = ptx::mbar_wait_cycles(dempty_u + 8 * dd.s, dd.parity ^ 1u, kWait);
-                        if (!ok) break;
+            const uint32_t half = (uint32_t)xhalf >> 4;  // descriptors count 16 bytes
+            const int my_steps = first < total ? ((total - first + stride - 1) / stride) * steps : 0;
+            for (int it = 0; it < my_steps && ok; ++it) {
+                const uint64_t bd = desc0 + (uint64_t)((uint32_t)(r.s * stage_bytes) >> 4);
+                const uint32_t at = tbase + acol + (uint32_t)(aa.s * kACols);
+#pragma unroll
+                for (int g = 0; g < GPS; ++g) {
+                    ok = ok && ptx::mbar_wait_cycles(dempty_u + 8 * dd.s, dd.parity ^ 1u, kWait);
+                    if (g == 0) ok = ok && ptx::mbar_wait_cycles(afull_u + 8 * aa.s, aa.parity, kWait);
+                    if (ok) {
                         ptx::tc_fence_after_sync();
-                        dt = tbase + (uint32_t)(dd.s * C::kRows);
-                    }
-                    ptx::umma_f16_ta(dt, at + 16, bd + 4, idesc, G32 ? 0u : 1u);
-                    ptx::umma_f16_ta(dt, at + 24, bd + 6, idesc, 1u);
-                    ptx::umma_commit(aempty_u + 8 * aa.s);
-                    ptx::umma_commit(empty_u + 8 * r.s);
-                    if (++in_group == gsteps || i + 1 == steps) {
+                        const uint32_t dt = tbase + (uint32_t)(dd.s * C::kRows);
+#pragma unroll
+                        for (int j = 0; j < 8 / GPS; ++j) {
+                            const int ks = g * (8 / GPS) + j;  // 16 rows of K
+                            ptx::umma_f16_ta(dt, at + (uint32_t)(8 * ks), bd + (ks >> 2) * half + (ks & 3) * 2, idesc,
+                                             j == 0 ? 0u : 1u);
+                        }
                         ptx::umma_commit(dfull_u + 8 * dd.s);
                         dd.advance(1, 2);
-                        in_group = 0;
                     }
-                    r.advance(1, NS);
-                    aa.advance(1, kNA);
                 }
+                if (ok) ptx::umma_commit(empty_u + 8 * r.s);
+                r.advance(1, NS);
+                aa.advance(1, kNA);
             }
             // every UMMA issued is complete before TMEM is freed
             ptx::umma_commit(done_u);
             ptx::mbar_wait_cycles(done_u, 0u, kWait);
         }
     } else if (warp >= C::kDW) {
-        // ---- converters: set c takes steps c, c + kConvSets, ... ----
+        // ---- converters: both halves of every step, or (two sets) one ----
         const int set = (warp - C::kDW) >> 2, q = warp & 3;
         const int n64 = (q & 1) * 32 + lane;
-        const uint8_t *raw0 = smem + xbytes + (q >> 1) * lin::kHalfBytes;
+        const uint8_t *raw0 = smem + 2 * xhalf + (q >> 1) * 2 * lin::kHalfBytes;
         const uint32_t at0 = tbase + ((uint32_t)(32 * q) << 16) + acol;
-        const int my_tiles = first < total ? (total - first + stride - 1) / stride : 0;
-        const int all = my_tiles * steps;
-        Ring r, aa;
-        r.s = aa.s = set;
-        for (int it = set; it < all; it += C::kConvSets) {
-            const bool ok = ptx::mbar_wait_cycles(full_u + 8 * r.s, r.parity, kWait) &&
-                            ptx::mbar_wait_cycles(aempty_u + 8 * aa.s, aa.parity ^ 1u, kWait);
+        const int my_steps = first < total ? ((total - first + stride - 1) / stride) * steps : 0;
+        Ring r, aa, old;  // the step's stage and A stage; the stage of the step that used the A stage before
+        for (int it = 0; it < my_steps; ++it) {
+            bool ok = ptx::mbar_wait_cycles(full_u + 8 * r.s, r.parity, kWait);
+            if (it >= kNA) {
+                ok = ok && ptx::mbar_wait_cycles(empty_u + 8 * old.s, old.parity, kWait);
+                old.advance(1, NS);
+            }
             if (!__all_sync(0xffffffffu, ok)) break;
             ptx::tc_fence_after_sync();
-            const uint8_t *raw = raw0 + r.s * stage_bytes;
-            uint32_t f[32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(raw + c * 1024 + ((n64 ^ (2 * c)) << 4));
-                lin::to_h4(v.x, f[4 * c], f[4 * c + 1]);
-                lin::to_h4(v.y, f[4 * c + 2], f[4 * c + 3]);
-                lin::to_h4(v.z, f[16 + 4 * c], f[16 + 4 * c + 1]);
-                lin::to_h4(v.w, f[16 + 4 * c + 2], f[16 + 4 * c + 3]);
+            for (int hh = 0; hh < 2 / C::kConvSets; ++hh) {
+                const int h = C::kConvSets == 2 ? set : hh;
+                const uint8_t *raw = raw0 + r.s * stage_bytes + h * lin::kHalfBytes;
+                uint32_t f[32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(raw + c * 1024 + ((n64 ^ (2 * c)) << 4));
+                    lin::to_h4(v.x, f[4 * c], f[4 * c + 1]);
+                    lin::to_h4(v.y, f[4 * c + 2], f[4 * c + 3]);
+                    lin::to_h4(v.z, f[16 + 4 * c], f[16 + 4 * c + 1]);
+                    lin::to_h4(v.w, f[16 + 4 * c + 2], f[16 + 4 * c + 3]);
+                }
+                ptx::tmem_st32(at0 + (uint32_t)(aa.s * kACols + h * 32), f);
             }
-            ptx::tmem_st32(at0 + (uint32_t)(aa.s * 32), f);
             ptx::tmem_wait_st();
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) {
-                ptx::mbar_arrive(afull_u + 8 * aa.s);
-                ptx::mbar_arrive(empty_u + 8 * r.s);
-            }
-            r.advance(C::kConvSets, NS);
-            aa.advance(C::kConvSets, kNA);
+            if (lane == 0) ptx::mbar_arrive(afull_u + 8 * aa.s);
+            r.advance(1, NS);
+            aa.advance(1, kNA);
         }
     } else {
         // ---- drains ----
@@ -372,25 +364,34 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             const TilePos p = tile_pos(t, ntiles, nrt);
             const int t64 = 2 * p.nt + (q >> 1);
             // this column's scales, one per group (a tile's missing second half: any)
-            const int gsub = lin::kBlockK / a.group;  // groups of a block
             const uint8_t *sp = static_cast<const uint8_t *>(a.packed) +
                                 ((long long)(t64 < tiles64 ? t64 : 0) * nblocks + b0) * unit + 2 * lin::kHalfBytes +
                                 (col & 63) * 2;
             int sub = 0;
             auto next_scale = [&]() -> float {
                 const float v = __half2float(__ushort_as_half(__ldg(reinterpret_cast<const unsigned short *>(sp))));
-                if (++sub == gsub) {
+                if (GPS == 1 || ++sub == GPS) {
                     sub = 0;
-                    sp += unit - (gsub - 1) * (lin::kTileN * 2);
+                    sp += unit - (GPS - 1) * (lin::kTileN * 2);
                 } else {
                     sp += lin::kTileN * 2;
                 }
                 return v;
             };
+            const long long row0 = (long long)p.rt * RT + row_off, packed0 = (long long)p.nt * kM + 32 * q;
+            const int nrows = (int)max(0ll, min((long long)per, a.rows - row0));
+            // residuals by 16 bytes where the addresses allow it
+            const __half *res = static_cast<const __half *>(a.residual) + row0 * a.residual_stride + packed0;
+            const bool vec_res = a.residual && packed0 + 32 <= a.n && a.residual_stride % 8 == 0 &&
+                                 (reinterpret_cast<uintptr_t>(a.residual) & 15) == 0;
+            if (vec_res)  // on their way to L2 while the tile is computed
+                for (int r = lane; r < nrows; r += 32)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(res + (long long)r * a.residual_stride));
             uint64_t acc[C::kAcc / 2];  // pairs of rows
 #pragma unroll
             for (int i = 0; i < C::kAcc / 2; ++i) acc[i] = 0ull;
             float sc = next_scale();
+            const int ngroups = steps * GPS;
             for (int g = 0; g < ngroups; ++g, dd.advance(1, 2)) {
                 const uint64_t s2 = ptx::f2_pack(sc, sc);
                 if (g + 1 < ngroups) sc = next_scale();
@@ -433,8 +434,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 break;
             }
             // ---- epilogue: 16 rows at a time through shared memory ----
-            const long long row0 = (long long)p.rt * RT + row_off;
-            const int nrows = (int)min((long long)per, a.rows - row0);
+            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+            uint4 q0 = zero, q1 = zero;
+            auto load_res = [&](int c) {
+                const int r = c * 16 + (lane >> 1);
+                if (vec_res && r < nrows) {
+                    const uint4 *src = reinterpret_cast<const uint4 *>(res + (long long)r * a.residual_stride + (lane & 1) * 16);
+                    q0 = src[0];
+                    q1 = src[1];
+                }
+            };
+            load_res(0);
 #pragma unroll
             for (int c = 0; c < C::kAcc / 16; ++c) {
                 if (c * 16 < nrows) {
@@ -446,7 +456,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                         st[(2 * i + 1) * kOutPitch + lane] = v1;
                     }
                     __syncwarp();
-                    write_rows(a, st, lane, row0 + c * 16, min(16, nrows - c * 16), (long long)p.nt * kM + 32 * q);
+                    const uint4 p0 = q0, p1 = q1;
+                    load_res(c + 1);  // the next rows' residuals
+                    if (a.gated)
+                        write_rows_act<true>(a, st, lane, row0 + c * 16, min(16, nrows - c * 16), packed0, false, p0, p1);
+                    else
+                        write_rows_act<false>(a, st, lane, row0 + c * 16, min(16, nrows - c * 16), packed0, vec_res, p0, p1);
                     __syncwarp();
                 }
             }
@@ -496,7 +511,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     }
 }
 
-template <typename C, bool G32>
+template <typename C, int GPS>
 cudaError_t launch_g(const LinearArgs &a, unsigned grid, cudaStream_t s) {
     static std::atomic<unsigned long long> done{0};  // devices whose shared-memory limit is set
     int dev = 0;
@@ -504,7 +519,7 @@ cudaError_t launch_g(const LinearArgs &a, unsigned grid, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(done.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(linear_tc_kernel<C, G32>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        e = cudaFuncSetAttribute(linear_tc_kernel<C, GPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
         if (e != cudaSuccess) return e;
         done.fetch_or(bit, std::memory_order_acq_rel);
     }
@@ -525,12 +540,12 @@ cudaError_t launch_g(const LinearArgs &a, unsigned grid, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, linear_tc_kernel<C, G32>, a, xmap);
+    return cudaLaunchKernelEx(&cfg, linear_tc_kernel<C, GPS>, a, xmap);
 }
 
 template <typename C>
 cudaError_t launch_t(const LinearArgs &a, unsigned grid, cudaStream_t s) {
-    return a.group == 32 ? launch_g<C, true>(a, grid, s) : launch_g<C, false>(a, grid, s);
+    return a.group == 32 ? launch_g<C, 4>(a, grid, s) : a.group == 64 ? launch_g<C, 2>(a, grid, s) : launch_g<C, 1>(a, grid, s);
 }
 
 // At most 14 warps of 144 registers per SM. Few rows: the weight stream asks
