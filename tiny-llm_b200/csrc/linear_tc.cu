@@ -87,6 +87,18 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
                    "=r"(r[15])
                  : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint64_t *p) {
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        r[2 * i] = (uint32_t)p[i];
+        r[2 * i + 1] = (uint32_t)(p[i] >> 32);
+    }
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                 "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 // Waits for this thread's TMEM loads; r is read after it.
 __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -120,12 +132,10 @@ struct Ring {
 };
 
 // One drain warp's [16 rows][32 packed columns] of sums, in shared memory, to
-// the output: lane = (row, half of the columns). A function of its own,
-// called for every 16 rows: inlined into the unrolled loop over a thread's
-// rows its activations alone outgrow the instruction cache (94,000 cycles a
-// tile against a few thousand). q0, q1: the lane's residuals where `have_res`.
+// the output: lane = (row, half of the columns). q0, q1: the lane's residuals
+// where `have_res`.
 template <int ACT, bool GATED>
-__device__ __noinline__ void write_rows(const LinearArgs &a, const float *st, int lane, long long row0, int nrows,
+__device__ __forceinline__ void write_rows(const LinearArgs &a, const float *st, int lane, long long row0, int nrows,
                                         long long packed0, bool have_res, uint4 q0, uint4 q1) {
     constexpr int W = GATED ? 8 : 16;  // outputs of the lane
     const int r = lane >> 1, h = lane & 1;
@@ -368,8 +378,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                                 ((long long)(t64 < tiles64 ? t64 : 0) * nblocks + b0) * unit + 2 * lin::kHalfBytes +
                                 (col & 63) * 2;
             int sub = 0;
-            auto next_scale = [&]() -> float {
-                const float v = __half2float(__ushort_as_half(__ldg(reinterpret_cast<const unsigned short *>(sp))));
+            auto next_scale = [&]() -> unsigned short {  // converted where it is used, a group after it was asked for
+                const unsigned short v = __ldg(reinterpret_cast<const unsigned short *>(sp));
                 if (GPS == 1 || ++sub == GPS) {
                     sub = 0;
                     sp += unit - (GPS - 1) * (lin::kTileN * 2);
@@ -390,14 +400,16 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             uint64_t acc[C::kAcc / 2];  // pairs of rows
 #pragma unroll
             for (int i = 0; i < C::kAcc / 2; ++i) acc[i] = 0ull;
-            float sc = next_scale();
+            unsigned short sc = next_scale();
             const int ngroups = steps * GPS;
             for (int g = 0; g < ngroups; ++g, dd.advance(1, 2)) {
-                const uint64_t s2 = ptx::f2_pack(sc, sc);
+                const unsigned short sraw = sc;
                 if (g + 1 < ngroups) sc = next_scale();
                 ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait_cycles(dfull_u + 8 * dd.s, dd.parity, kWait));
                 if (!ok) continue;
                 ptx::tc_fence_after_sync();
+                const float sf = __half2float(__ushort_as_half(sraw));
+                const uint64_t s2 = ptx::f2_pack(sf, sf);
 #pragma unroll
                 for (int c = 0; c < C::kAcc / 16; ++c) {
                     if (c * 16 < per) {
@@ -411,6 +423,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                                             acc[c * 8 + i]);
                     }
                 }
+                if (g + 1 == ngroups && csplit == 1) break;  // the accumulator stays until the tile is written
                 ptx::tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(dempty_u + 8 * dd.s);
@@ -433,7 +446,16 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 }
                 break;
             }
-            // ---- epilogue: 16 rows at a time through shared memory ----
+            // ---- epilogue: the sums back to the last group's accumulator, then
+            // 16 rows at a time through shared memory, in a loop that is not
+            // unrolled: from registers it would have to be, and its code with
+            // the activations then outgrows the instruction cache (94,000
+            // cycles a tile) ----
+            const uint32_t tsum = tlane + (uint32_t)(dd.s * C::kRows);
+#pragma unroll
+            for (int c = 0; c < C::kAcc / 16; ++c)
+                if (c * 16 < per) tmem_st16(tsum + (uint32_t)(c * 16), acc + c * 8);
+            ptx::tmem_wait_st();
             const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
             uint4 q0 = zero, q1 = zero;
             auto load_res = [&](int c) {
@@ -445,26 +467,26 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 }
             };
             load_res(0);
+#pragma unroll 1
+            for (int c = 0; c * 16 < nrows; ++c) {
+                uint32_t v[16];
+                tmem_ld16(tsum + (uint32_t)(c * 16), v);
+                tmem_wait_ld16(v);
 #pragma unroll
-            for (int c = 0; c < C::kAcc / 16; ++c) {
-                if (c * 16 < nrows) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float v0, v1;
-                        ptx::f2_unpack(acc[c * 8 + i], v0, v1);
-                        st[(2 * i) * kOutPitch + lane] = v0;
-                        st[(2 * i + 1) * kOutPitch + lane] = v1;
-                    }
-                    __syncwarp();
-                    const uint4 p0 = q0, p1 = q1;
-                    load_res(c + 1);  // the next rows' residuals
-                    if (a.gated)
-                        write_rows_act<true>(a, st, lane, row0 + c * 16, min(16, nrows - c * 16), packed0, false, p0, p1);
-                    else
-                        write_rows_act<false>(a, st, lane, row0 + c * 16, min(16, nrows - c * 16), packed0, vec_res, p0, p1);
-                    __syncwarp();
-                }
+                for (int i = 0; i < 16; ++i) st[i * kOutPitch + lane] = __uint_as_float(v[i]);
+                __syncwarp();
+                const uint4 p0 = q0, p1 = q1;
+                load_res(c + 1);  // the next rows' residuals
+                if (a.gated)
+                    write_rows_act<true>(a, st, lane, row0 + c * 16, min(16, nrows - c * 16), packed0, false, p0, p1);
+                else
+                    write_rows_act<false>(a, st, lane, row0 + c * 16, min(16, nrows - c * 16), packed0, vec_res, p0, p1);
+                __syncwarp();
             }
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(dempty_u + 8 * dd.s);
+            dd.advance(1, 2);
         }
     }
 
