@@ -3,7 +3,7 @@
 // linear.cu takes. Same operation, same packed weights (linear_pack.cuh).
 //
 // The packed weight columns are the M side of the UMMA (128 per tile: two
-// tiles of 64 of the packed layout), a tile of up to 192 batch rows the N
+// tiles of 64 of the packed layout), a tile of up to 160 batch rows the N
 // side, K in steps of 128 (a block of the packed layout). The int8 weights
 // become the fp16 A operand on the way, exactly and in TMEM; their scales
 // multiply the fp32 sums of one scale group, so no weight is rounded and no
@@ -14,9 +14,9 @@
 //   converters  thread = weight column: 64 bytes from shared memory, to 64
 //               fp16, one tcgen05.st of 32 columns: the K-major A operand of
 //               half a step (four warps do both halves, eight one each);
-//   MMA         one thread: eight UMMAs (K = 16) per step, A in TMEM, B in
-//               shared memory, into one of two accumulators, changed with
-//               every scale group;
+//   MMA         one thread each of two warps: eight UMMAs (K = 16) per step, A
+//               in TMEM, B in shared memory; the scale groups take two
+//               accumulators in turn, each with an issuing warp of its own;
 //   drains      thread = weight column (TMEM lane): when a group is complete,
 //               acc += scale * sum for the thread's rows, in registers; after
 //               the last group the epilogue from them.
@@ -24,11 +24,12 @@
 // filled meanwhile), and the CTAs are persistent: the next tile's first
 // groups run while a tile's outputs are written.
 //
-// What bounds it is the MMA thread: a wait that succeeds at once costs it
-// about 110 cycles, a commit 80, a UMMA 75 or its pipe time (rows / 2). So a
-// step is as deep as the layout's block, the stage and the A operand are
-// released by one commit, and the thread does not wait for the activations:
-// the converters waited for the same barrier before they arrived.
+// A wait that succeeds at once costs an issuing thread about 110 cycles, a
+// commit 80, a UMMA 75 or its pipe time (rows / 2) while the pipe's queue is
+// full. So a step is as deep as the layout's block, the stage and the A
+// operand are released by one commit, the issuing threads do not wait for the
+// activations (the converters waited for the same barrier before they
+// arrived), and one thread's waits pass while the other's UMMAs run.
 //
 // Too few tiles for the SMs: a cluster's CTAs share a tile's K and add their
 // sums in distributed shared memory, in rank order. No atomics, no workspace:
@@ -69,11 +70,11 @@ template <int kRows_, int kCW_, int kDW_, int kPerSm_>
 struct Cfg {
     static constexpr int kRows = kRows_, kCW = kCW_, kDW = kDW_, kPerSm = kPerSm_;
     static constexpr int kConvSets = kCW / 4, kDrainSets = kDW / 4;
-    static constexpr int kProd = kDW + kCW, kMma = kProd + 1;  // warps
-    static constexpr int kThreads = 32 * (kDW + kCW + 2);
+    static constexpr int kProd = kDW + kCW, kMma = kProd + 1;  // warps; two issue UMMAs
+    static constexpr int kThreads = 32 * (kDW + kCW + 3);
     static constexpr int kAcc = kRows / kDrainSets;  // rows per drain thread
     static constexpr uint32_t kTmemCols = 2 * kRows + kNA * kACols <= 256 ? 256 : 512;
-    static constexpr int kRing = (kPerSm == 2 ? 96 : 192) * 1024;
+    static constexpr int kRing = (kPerSm == 2 ? 96 : kDW > 12 ? 176 : 192) * 1024;
     static constexpr int kOut = kDW * kOutRows * kOutPitch * 4;  // the drain warps' rows on their way out
     static constexpr int kBars = (2 * kMaxStages + kNA + 5) * 8;
     static constexpr int kSmem = 1024 + kRing + kOut + kBars + 16;
@@ -87,13 +88,10 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
                    "=r"(r[15])
                  : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint64_t *p) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float *p) {
     uint32_t r[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        r[2 * i] = (uint32_t)p[i];
-        r[2 * i + 1] = (uint32_t)(p[i] >> 32);
-    }
+    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(p[i]);
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
                  "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
@@ -226,14 +224,14 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMaxStages; ++s) {
             ptx::mbar_init(full_u + 8 * s, 1);
-            ptx::mbar_init(empty_u + 8 * s, 1);
+            ptx::mbar_init(empty_u + 8 * s, GPS == 1 ? 1 : 2);  // commits: of the warp(s) that had a part of the step
         }
         for (int s = 0; s < kNA; ++s) ptx::mbar_init(afull_u + 8 * s, C::kCW);
         for (int s = 0; s < 2; ++s) {
             ptx::mbar_init(dfull_u + 8 * s, 1);
             ptx::mbar_init(dempty_u + 8 * s, C::kDW);
         }
-        ptx::mbar_init(done_u, 1);
+        ptx::mbar_init(done_u, 2);
         ptx::fence_barrier_init();
     }
     if (warp == C::kMma) ptx::tmem_alloc(ptx::smem_u32(&s_tmem), C::kTmemCols);
@@ -284,38 +282,43 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 for (int i = max(0, issued - NS); i < issued; ++i)
                     ptx::mbar_wait_cycles(full_u + 8 * (i % NS), (uint32_t)((i / NS) & 1), kWait);
         }
-    } else if (warp == C::kMma) {
+    } else if (warp >= C::kMma) {
         if (lane == 0) {
-            // ---- UMMA issue ----
+            // ---- UMMA issue: warp m has accumulator m, every second group ----
+            const int m = warp - C::kMma;
             const uint32_t idesc = (1u << 4) | ((uint32_t)(RT >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
             const uint64_t desc0 = ptx::umma_desc_sw128(ptx::smem_u32(smem), 16, 1024);
-            Ring r, aa, dd;  // ring stage, A stage, accumulator
-            bool ok = true;
             const uint32_t half = (uint32_t)xhalf >> 4;  // descriptors count 16 bytes
             const int my_steps = first < total ? ((total - first + stride - 1) / stride) * steps : 0;
-            for (int it = 0; it < my_steps && ok; ++it) {
+            const uint32_t dt = tbase + (uint32_t)(m * C::kRows), dfull = dfull_u + 8 * m, dempty = dempty_u + 8 * m;
+            constexpr int kBy = GPS == 1 ? 2 : 1;  // steps from one with a group of this warp to the next
+            Ring r, aa;
+            r.s = GPS == 1 ? m : 0;
+            aa.s = r.s;
+            uint32_t dpar = 1;
+            bool ok = true;
+            for (int it = r.s; it < my_steps && ok; it += kBy) {
                 const uint64_t bd = desc0 + (uint64_t)((uint32_t)(r.s * stage_bytes) >> 4);
                 const uint32_t at = tbase + acol + (uint32_t)(aa.s * kACols);
+                ok = ptx::mbar_wait_cycles(afull_u + 8 * aa.s, aa.parity, kWait);
 #pragma unroll
-                for (int g = 0; g < GPS; ++g) {
-                    ok = ok && ptx::mbar_wait_cycles(dempty_u + 8 * dd.s, dd.parity ^ 1u, kWait);
-                    if (g == 0) ok = ok && ptx::mbar_wait_cycles(afull_u + 8 * aa.s, aa.parity, kWait);
-                    if (ok) {
-                        ptx::tc_fence_after_sync();
-                        const uint32_t dt = tbase + (uint32_t)(dd.s * C::kRows);
+                for (int gg = 0; gg < (GPS + 1) / 2; ++gg) {
+                    ok = ok && ptx::mbar_wait_cycles(dempty, dpar, kWait);
+                    if (!ok) break;
+                    dpar ^= 1u;
+                    ptx::tc_fence_after_sync();
+                    const int ks0 = GPS == 1 ? 0 : (2 * gg + m) * (8 / GPS);  // the group's first 16 rows of K
 #pragma unroll
-                        for (int j = 0; j < 8 / GPS; ++j) {
-                            const int ks = g * (8 / GPS) + j;  // 16 rows of K
-                            ptx::umma_f16_ta(dt, at + (uint32_t)(8 * ks), bd + (ks >> 2) * half + (ks & 3) * 2, idesc,
-                                             j == 0 ? 0u : 1u);
-                        }
-                        ptx::umma_commit(dfull_u + 8 * dd.s);
-                        dd.advance(1, 2);
+                    for (int j = 0; j < 8 / GPS; ++j) {
+                        const int ks = ks0 + j;
+                        ptx::umma_f16_ta(dt, at + (uint32_t)(8 * ks), bd + (uint32_t)(ks >> 2) * half + (uint32_t)(ks & 3) * 2,
+                                         idesc, j == 0 ? 0u : 1u);
                     }
+                    ptx::umma_commit(dfull);
                 }
                 if (ok) ptx::umma_commit(empty_u + 8 * r.s);
-                r.advance(1, NS);
-                aa.advance(1, kNA);
+                r.advance(kBy, NS);
+                aa.advance(kBy, kNA);
             }
             // every UMMA issued is complete before TMEM is freed
             ptx::umma_commit(done_u);
@@ -370,13 +373,22 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         Ring dd;
         bool ok = true;
         ptx::griddep_wait();
+        const bool res_vec = a.residual && a.residual_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.residual) & 15) == 0;
         for (int t = first; t < total; t += stride) {
-            const TilePos p = tile_pos(t, ntiles, nrt);
-            const int t64 = 2 * p.nt + (q >> 1);
-            // this column's scales, one per group (a tile's missing second half: any)
-            const uint8_t *sp = static_cast<const uint8_t *>(a.packed) +
-                                ((long long)(t64 < tiles64 ? t64 : 0) * nblocks + b0) * unit + 2 * lin::kHalfBytes +
-                                (col & 63) * 2;
+            const uint8_t *sp;
+            {
+                // this column's scales, one per group (a tile's missing second half: any)
+                const TilePos p = tile_pos(t, ntiles, nrt);
+                const int t64 = 2 * p.nt + (q >> 1);
+                sp = static_cast<const uint8_t *>(a.packed) + ((long long)(t64 < tiles64 ? t64 : 0) * nblocks + b0) * unit +
+                     2 * lin::kHalfBytes + (col & 63) * 2;
+                // the residuals, on their way to L2 while the tile is computed
+                const long long row0 = (long long)p.rt * RT + row_off, packed0 = (long long)p.nt * kM + 32 * q;
+                if (res_vec && packed0 + 32 <= a.n)
+                    for (int r = lane; r < per && row0 + r < a.rows; r += 32)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const __half *>(a.residual) +
+                                                                      (row0 + r) * a.residual_stride + packed0));
+            }
             int sub = 0;
             auto next_scale = [&]() -> unsigned short {  // converted where it is used, a group after it was asked for
                 const unsigned short v = __ldg(reinterpret_cast<const unsigned short *>(sp));
@@ -388,18 +400,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 }
                 return v;
             };
-            const long long row0 = (long long)p.rt * RT + row_off, packed0 = (long long)p.nt * kM + 32 * q;
-            const int nrows = (int)max(0ll, min((long long)per, a.rows - row0));
-            // residuals by 16 bytes where the addresses allow it
-            const __half *res = static_cast<const __half *>(a.residual) + row0 * a.residual_stride + packed0;
-            const bool vec_res = a.residual && packed0 + 32 <= a.n && a.residual_stride % 8 == 0 &&
-                                 (reinterpret_cast<uintptr_t>(a.residual) & 15) == 0;
-            if (vec_res)  // on their way to L2 while the tile is computed
-                for (int r = lane; r < nrows; r += 32)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(res + (long long)r * a.residual_stride));
-            uint64_t acc[C::kAcc / 2];  // pairs of rows
+            float acc[C::kAcc];
 #pragma unroll
-            for (int i = 0; i < C::kAcc / 2; ++i) acc[i] = 0ull;
+            for (int i = 0; i < C::kAcc; ++i) acc[i] = 0.f;
             unsigned short sc = next_scale();
             const int ngroups = steps * GPS;
             for (int g = 0; g < ngroups; ++g, dd.advance(1, 2)) {
@@ -409,7 +412,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 if (!ok) continue;
                 ptx::tc_fence_after_sync();
                 const float sf = __half2float(__ushort_as_half(sraw));
-                const uint64_t s2 = ptx::f2_pack(sf, sf);
 #pragma unroll
                 for (int c = 0; c < C::kAcc / 16; ++c) {
                     if (c * 16 < per) {
@@ -417,10 +419,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                         tmem_ld16(tlane + (uint32_t)(dd.s * C::kRows + c * 16), v);
                         tmem_wait_ld16(v);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            acc[c * 8 + i] =
-                                ptx::f2_fma(ptx::f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), s2,
-                                            acc[c * 8 + i]);
+                        for (int i = 0; i < 16; ++i)
+                            acc[c * 16 + i] = fmaf(__uint_as_float(v[i]), sf, acc[c * 16 + i]);
                     }
                 }
                 if (g + 1 == ngroups && csplit == 1) break;  // the accumulator stays until the tile is written
@@ -431,19 +431,13 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             if (!ok) {
                 const float nan = __int_as_float(0x7fffffff);
 #pragma unroll
-                for (int i = 0; i < C::kAcc / 2; ++i) acc[i] = ptx::f2_pack(nan, nan);
+                for (int i = 0; i < C::kAcc; ++i) acc[i] = nan;
             }
             if (csplit > 1) {  // the CTA's one tile: its sums to the ring (every step is consumed)
                 float *part = reinterpret_cast<float *>(smem);
 #pragma unroll
-                for (int i = 0; i < C::kAcc / 2; ++i) {
-                    if (2 * i < per) {
-                        float v0, v1;
-                        ptx::f2_unpack(acc[i], v0, v1);
-                        part[(row_off + 2 * i) * kM + col] = v0;
-                        part[(row_off + 2 * i + 1) * kM + col] = v1;
-                    }
-                }
+                for (int i = 0; i < C::kAcc; ++i)
+                    if (i < per) part[(row_off + i) * kM + col] = acc[i];
                 break;
             }
             // ---- epilogue: the sums back to the last group's accumulator, then
@@ -451,10 +445,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             // unrolled: from registers it would have to be, and its code with
             // the activations then outgrows the instruction cache (94,000
             // cycles a tile) ----
+            int t_again = t;  // (the tile's place computed anew: kept, it would cost the loop above its registers)
+            asm volatile("" : "+r"(t_again));
+            const TilePos p = tile_pos(t_again, ntiles, nrt);
+            const long long row0 = (long long)p.rt * RT + row_off, packed0 = (long long)p.nt * kM + 32 * q;
+            const int nrows = (int)max(0ll, min((long long)per, a.rows - row0));
+            const __half *res = static_cast<const __half *>(a.residual) + row0 * a.residual_stride + packed0;
+            const bool vec_res = res_vec && packed0 + 32 <= a.n;  // residuals by 16 bytes
             const uint32_t tsum = tlane + (uint32_t)(dd.s * C::kRows);
 #pragma unroll
             for (int c = 0; c < C::kAcc / 16; ++c)
-                if (c * 16 < per) tmem_st16(tsum + (uint32_t)(c * 16), acc + c * 8);
+                if (c * 16 < per) tmem_st16(tsum + (uint32_t)(c * 16), acc + c * 16);
             ptx::tmem_wait_st();
             const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
             uint4 q0 = zero, q1 = zero;
@@ -571,10 +572,10 @@ cudaError_t launch_t(const LinearArgs &a, unsigned grid, cudaStream_t s) {
 }
 
 // At most 14 warps of 144 registers per SM. Few rows: the weight stream asks
-// for converters; many: the sums ask for drains (96 rows a thread).
+// for converters; many: the sums ask for drains (80 rows a thread; 96 measured slower).
 using Small = Cfg<32, 4, 4, 2>;
 using Medium = Cfg<64, 8, 4, 1>;
-using Large = Cfg<192, 4, 8, 1>;
+using Large = Cfg<160, 4, 8, 1>;
 
 }  // namespace
 
