@@ -89,13 +89,21 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const
         s_failed = 0;
     }
     __syncthreads();
+    // Programmatic dependent launch: the next kernel's CTAs may come as ours
+    // leave. Until the kernel before has completed they only ask L2 for their
+    // first weights (a prefetch: a later write of them still wins) and sleep.
     ptx::griddep_launch_dependents();
+    const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)tile * nblocks + b0) * unit;
+    if (warp == kConsumers && lane == 0) {
+        ptx::prefetch_tensormap(&xmap);
+        ptx::bulk_prefetch_l2(w, (uint32_t)(min(C::kNS, count) * unit));
+    }
+    __syncwarp();
+    ptx::griddep_wait();
 
     if (warp == kConsumers) {
         // ---- producer (one lane) ----
-        ptx::griddep_wait();
         if (lane == 0) {
-            const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)tile * nblocks + b0) * unit;
             const uint64_t once = ptx::l2_policy_evict_first(), keep = ptx::l2_policy_evict_last();
             int issued = 0;
             for (int i = 0; i < count; ++i, ++issued) {
@@ -217,7 +225,6 @@ __global__ void __launch_bounds__(kThreads, RB >= 4 ? 1 : 2) linear_kernel(const
     }
     cg::cluster_group cluster = cg::this_cluster();
     if (csplit > 1) cluster.sync();
-    ptx::griddep_wait();
     auto total = [&](int r, int c) {
         if (csplit == 1) return part[r * C::kRowF + c];
         float v = 0.f;

@@ -3,7 +3,7 @@
 // linear.cu takes. Same operation, same packed weights (linear_pack.cuh).
 //
 // The packed weight columns are the M side of the UMMA (128 per tile: two
-// tiles of 64 of the packed layout), a tile of up to 160 batch rows the N
+// tiles of 64 of the packed layout), a tile of up to 128 batch rows the N
 // side, K in steps of 128 (a block of the packed layout). The int8 weights
 // become the fp16 A operand on the way, exactly and in TMEM; their scales
 // multiply the fp32 sums of one scale group, so no weight is rounded and no
@@ -52,7 +52,6 @@ namespace cg = cooperative_groups;
 
 constexpr int kM = 128;            // packed columns of a tile
 constexpr int kStepK = lin::kBlockK;  // rows of K per ring stage
-constexpr int kNA = 2;             // A operand stages in TMEM
 constexpr int kACols = kStepK / 2;  // TMEM columns of one (fp16 pairs along K)
 constexpr int kRaw = 2 * 2 * lin::kHalfBytes;  // packed weights of a step
 constexpr int kMaxStages = 8;
@@ -64,20 +63,25 @@ struct alignas(64) Map {  // a tensor map, opaque here
     unsigned char bytes[128];
 };
 
-// kRows: most rows of a tile. kCW, kDW: converter and drain warps (sets of
-// four, one per TMEM lane quarter). kPerSm: CTAs per SM.
-template <int kRows_, int kCW_, int kDW_, int kPerSm_>
+// kRows: most rows of a tile. kNA: A operand stages in TMEM. kCW, kDW: converter and drain warps (sets of
+// four, one per TMEM lane quarter). kIssue: warps that issue UMMAs. kPerSm:
+// CTAs per SM.
+template <int kRows_, int kNA_, int kCW_, int kDW_, int kIssue_, int kPerSm_>
 struct Cfg {
+    static constexpr int kNA = kNA_;
+    static constexpr int kIssue = kIssue_;
     static constexpr int kRows = kRows_, kCW = kCW_, kDW = kDW_, kPerSm = kPerSm_;
     static constexpr int kConvSets = kCW / 4, kDrainSets = kDW / 4;
-    static constexpr int kProd = kDW + kCW, kMma = kProd + 1;  // warps; two issue UMMAs
-    static constexpr int kThreads = 32 * (kDW + kCW + 3);
+    static constexpr int kProd = kDW + kCW, kMma = kProd + 1;  // warps
+    static constexpr int kThreads = 32 * (kDW + kCW + 1 + kIssue);
     static constexpr int kAcc = kRows / kDrainSets;  // rows per drain thread
     static constexpr uint32_t kTmemCols = 2 * kRows + kNA * kACols <= 256 ? 256 : 512;
     static constexpr int kRing = (kPerSm == 2 ? 96 : kDW > 12 ? 176 : 192) * 1024;
     static constexpr int kOut = kDW * kOutRows * kOutPitch * 4;  // the drain warps' rows on their way out
     static constexpr int kBars = (2 * kMaxStages + kNA + 5) * 8;
     static constexpr int kSmem = 1024 + kRing + kOut + kBars + 16;
+    static_assert(kIssue == 1 || kNA % 2 == 0, "an issuing warp meets every phase of its A stages");
+    static_assert(kRing / (kRows * 256 + kRaw) > kNA, "a converter meets every phase it waits for");
     static_assert(kAcc % 16 == 0 && kPerSm * kTmemCols <= 512, "tile");
 };
 
@@ -201,8 +205,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing + C::kOut);
     const uint32_t full_u = ptx::smem_u32(bars);           // [stages] weights and activations landed
     const uint32_t empty_u = full_u + 8 * kMaxStages;      // [stages] multiplied: the stage and its A operand are free
-    const uint32_t afull_u = empty_u + 8 * kMaxStages;     // [kNA] A operand in TMEM
-    const uint32_t dfull_u = afull_u + 8 * kNA;            // [2] a group's sums complete
+    const uint32_t afull_u = empty_u + 8 * kMaxStages;     // [C::kNA] A operand in TMEM
+    const uint32_t dfull_u = afull_u + 8 * C::kNA;            // [2] a group's sums complete
     const uint32_t dempty_u = dfull_u + 16;                // [2] ... and drained
     const uint32_t done_u = dempty_u + 16;                 // every UMMA complete
     __shared__ uint32_t s_tmem;
@@ -219,19 +223,19 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     const int steps = b1 - b0;
     const int first = blockIdx.x / csplit, stride = gridDim.x / csplit;
     const int xhalf = RT * 128, stage_bytes = 2 * xhalf + kRaw;
-    const int NS = min(kMaxStages, C::kRing / stage_bytes);  // > kNA: a converter meets every phase it waits for
+    const int NS = min(kMaxStages, C::kRing / stage_bytes);  // > C::kNA: a converter meets every phase it waits for
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMaxStages; ++s) {
             ptx::mbar_init(full_u + 8 * s, 1);
-            ptx::mbar_init(empty_u + 8 * s, GPS == 1 ? 1 : 2);  // commits: of the warp(s) that had a part of the step
+            ptx::mbar_init(empty_u + 8 * s, GPS == 1 ? 1 : C::kIssue);  // commits: of the warp(s) that had a part of the step
         }
-        for (int s = 0; s < kNA; ++s) ptx::mbar_init(afull_u + 8 * s, C::kCW);
+        for (int s = 0; s < C::kNA; ++s) ptx::mbar_init(afull_u + 8 * s, C::kCW);
         for (int s = 0; s < 2; ++s) {
             ptx::mbar_init(dfull_u + 8 * s, 1);
             ptx::mbar_init(dempty_u + 8 * s, C::kDW);
         }
-        ptx::mbar_init(done_u, 2);
+        ptx::mbar_init(done_u, C::kIssue);
         ptx::fence_barrier_init();
     }
     if (warp == C::kMma) ptx::tmem_alloc(ptx::smem_u32(&s_tmem), C::kTmemCols);
@@ -247,7 +251,17 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     if (warp == C::kProd) {
         if (lane == 0) {
             // ---- producer ----
+            // Programmatic dependent launch: until the kernel before has
+            // completed, only a prefetch of the first weights to L2 (a later
+            // write of them still wins).
             ptx::prefetch_tensormap(&xmap);
+            if (first < total) {
+                const TilePos p = tile_pos(first, ntiles, nrt);
+                const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)(2 * p.nt) * nblocks + b0) * unit;
+                const uint32_t bytes = (uint32_t)(min(NS, steps) * unit);
+                ptx::bulk_prefetch_l2(w, bytes);
+                if (2 * p.nt + 1 < tiles64) ptx::bulk_prefetch_l2(w + (long long)nblocks * unit, bytes);
+            }
             ptx::griddep_wait();
             const uint64_t keep = ptx::l2_policy_evict_last();
             const uint64_t wpol = nrt > 1 ? keep : ptx::l2_policy_evict_first();  // weights: read once per row tile
@@ -271,6 +285,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     ptx::mbar_arrive_expect_tx(bar, bytes);
                     ptx::bulk_load(dst + 2 * xhalf, w0, 2 * lin::kHalfBytes, bar, wpol);
                     if (both) ptx::bulk_load(dst + 2 * xhalf + 2 * lin::kHalfBytes, w1, 2 * lin::kHalfBytes, bar, wpol);
+                    // the block's scales, on their way to L2 for the drains: a
+                    // load of them is asked for one group ahead, less than HBM takes
+                    ptx::bulk_prefetch_l2(w0 + 2 * lin::kHalfBytes, (uint32_t)(unit - 2 * lin::kHalfBytes));
+                    if (both) ptx::bulk_prefetch_l2(w1 + 2 * lin::kHalfBytes, (uint32_t)(unit - 2 * lin::kHalfBytes));
                     const int k0 = (b0 + i) * kStepK;  // (a half past K lies wholly out of bounds: zeros)
                     ptx::tma_load_2d(dst, &xmap, bar, k0, p.rt * RT, keep);
                     ptx::tma_load_2d(dst + xhalf, &xmap, bar, k0 + 64, p.rt * RT, keep);
@@ -284,41 +302,43 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         }
     } else if (warp >= C::kMma) {
         if (lane == 0) {
-            // ---- UMMA issue: warp m has accumulator m, every second group ----
+            // ---- UMMA issue: one warp for all groups, or warp m of two for
+            // every second one, with accumulator m ----
             const int m = warp - C::kMma;
             const uint32_t idesc = (1u << 4) | ((uint32_t)(RT >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
             const uint64_t desc0 = ptx::umma_desc_sw128(ptx::smem_u32(smem), 16, 1024);
             const uint32_t half = (uint32_t)xhalf >> 4;  // descriptors count 16 bytes
             const int my_steps = first < total ? ((total - first + stride - 1) / stride) * steps : 0;
-            const uint32_t dt = tbase + (uint32_t)(m * C::kRows), dfull = dfull_u + 8 * m, dempty = dempty_u + 8 * m;
-            constexpr int kBy = GPS == 1 ? 2 : 1;  // steps from one with a group of this warp to the next
-            Ring r, aa;
-            r.s = GPS == 1 ? m : 0;
-            aa.s = r.s;
-            uint32_t dpar = 1;
+            constexpr int kBy = C::kIssue == 2 && GPS == 1 ? 2 : 1;          // steps from one of this warp's to the next
+            constexpr int kMine = C::kIssue == 2 ? (GPS + 1) / 2 : GPS;      // its groups of a step
+            Ring r, aa, dd;
+            r.s = aa.s = kBy == 2 ? m : 0;
+            dd.s = m;
             bool ok = true;
             for (int it = r.s; it < my_steps && ok; it += kBy) {
                 const uint64_t bd = desc0 + (uint64_t)((uint32_t)(r.s * stage_bytes) >> 4);
                 const uint32_t at = tbase + acol + (uint32_t)(aa.s * kACols);
-                ok = ptx::mbar_wait_cycles(afull_u + 8 * aa.s, aa.parity, kWait);
 #pragma unroll
-                for (int gg = 0; gg < (GPS + 1) / 2; ++gg) {
-                    ok = ok && ptx::mbar_wait_cycles(dempty, dpar, kWait);
+                for (int gg = 0; gg < kMine; ++gg) {
+                    ok = ok && ptx::mbar_wait_cycles(dempty_u + 8 * dd.s, dd.parity ^ 1u, kWait);
+                    if (gg == 0) ok = ok && ptx::mbar_wait_cycles(afull_u + 8 * aa.s, aa.parity, kWait);
                     if (!ok) break;
-                    dpar ^= 1u;
                     ptx::tc_fence_after_sync();
-                    const int ks0 = GPS == 1 ? 0 : (2 * gg + m) * (8 / GPS);  // the group's first 16 rows of K
+                    const uint32_t dt = tbase + (uint32_t)(dd.s * C::kRows);
+                    // the group's first 16 rows of K
+                    const int ks0 = (GPS == 1 ? 0 : C::kIssue == 2 ? 2 * gg + m : gg) * (8 / GPS);
 #pragma unroll
                     for (int j = 0; j < 8 / GPS; ++j) {
                         const int ks = ks0 + j;
                         ptx::umma_f16_ta(dt, at + (uint32_t)(8 * ks), bd + (uint32_t)(ks >> 2) * half + (uint32_t)(ks & 3) * 2,
                                          idesc, j == 0 ? 0u : 1u);
                     }
-                    ptx::umma_commit(dfull);
+                    ptx::umma_commit(dfull_u + 8 * dd.s);
+                    dd.advance(C::kIssue, 2);
                 }
                 if (ok) ptx::umma_commit(empty_u + 8 * r.s);
                 r.advance(kBy, NS);
-                aa.advance(kBy, kNA);
+                aa.advance(kBy, C::kNA);
             }
             // every UMMA issued is complete before TMEM is freed
             ptx::umma_commit(done_u);
@@ -334,7 +354,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         Ring r, aa, old;  // the step's stage and A stage; the stage of the step that used the A stage before
         for (int it = 0; it < my_steps; ++it) {
             bool ok = ptx::mbar_wait_cycles(full_u + 8 * r.s, r.parity, kWait);
-            if (it >= kNA) {
+            if (it >= C::kNA) {
                 ok = ok && ptx::mbar_wait_cycles(empty_u + 8 * old.s, old.parity, kWait);
                 old.advance(1, NS);
             }
@@ -360,7 +380,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(afull_u + 8 * aa.s);
             r.advance(1, NS);
-            aa.advance(1, kNA);
+            aa.advance(1, C::kNA);
         }
     } else {
         // ---- drains ----
@@ -373,22 +393,13 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         Ring dd;
         bool ok = true;
         ptx::griddep_wait();
-        const bool res_vec = a.residual && a.residual_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.residual) & 15) == 0;
         for (int t = first; t < total; t += stride) {
-            const uint8_t *sp;
-            {
-                // this column's scales, one per group (a tile's missing second half: any)
-                const TilePos p = tile_pos(t, ntiles, nrt);
-                const int t64 = 2 * p.nt + (q >> 1);
-                sp = static_cast<const uint8_t *>(a.packed) + ((long long)(t64 < tiles64 ? t64 : 0) * nblocks + b0) * unit +
-                     2 * lin::kHalfBytes + (col & 63) * 2;
-                // the residuals, on their way to L2 while the tile is computed
-                const long long row0 = (long long)p.rt * RT + row_off, packed0 = (long long)p.nt * kM + 32 * q;
-                if (res_vec && packed0 + 32 <= a.n)
-                    for (int r = lane; r < per && row0 + r < a.rows; r += 32)
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const __half *>(a.residual) +
-                                                                      (row0 + r) * a.residual_stride + packed0));
-            }
+            const TilePos p = tile_pos(t, ntiles, nrt);
+            const int t64 = 2 * p.nt + (q >> 1);
+            // this column's scales, one per group (a tile's missing second half: any)
+            const uint8_t *sp = static_cast<const uint8_t *>(a.packed) +
+                                ((long long)(t64 < tiles64 ? t64 : 0) * nblocks + b0) * unit + 2 * lin::kHalfBytes +
+                                (col & 63) * 2;
             int sub = 0;
             auto next_scale = [&]() -> unsigned short {  // converted where it is used, a group after it was asked for
                 const unsigned short v = __ldg(reinterpret_cast<const unsigned short *>(sp));
@@ -400,6 +411,15 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 }
                 return v;
             };
+            const long long row0 = (long long)p.rt * RT + row_off, packed0 = (long long)p.nt * kM + 32 * q;
+            const int nrows = (int)max(0ll, min((long long)per, a.rows - row0));
+            // residuals by 16 bytes where the addresses allow it
+            const __half *res = static_cast<const __half *>(a.residual) + row0 * a.residual_stride + packed0;
+            const bool vec_res = a.residual && packed0 + 32 <= a.n && a.residual_stride % 8 == 0 &&
+                                 (reinterpret_cast<uintptr_t>(a.residual) & 15) == 0;
+            if (vec_res)  // on their way to L2 while the tile is computed
+                for (int r = lane; r < nrows; r += 32)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(res + (long long)r * a.residual_stride));
             float acc[C::kAcc];
 #pragma unroll
             for (int i = 0; i < C::kAcc; ++i) acc[i] = 0.f;
@@ -445,13 +465,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
             // unrolled: from registers it would have to be, and its code with
             // the activations then outgrows the instruction cache (94,000
             // cycles a tile) ----
-            int t_again = t;  // (the tile's place computed anew: kept, it would cost the loop above its registers)
-            asm volatile("" : "+r"(t_again));
-            const TilePos p = tile_pos(t_again, ntiles, nrt);
-            const long long row0 = (long long)p.rt * RT + row_off, packed0 = (long long)p.nt * kM + 32 * q;
-            const int nrows = (int)max(0ll, min((long long)per, a.rows - row0));
-            const __half *res = static_cast<const __half *>(a.residual) + row0 * a.residual_stride + packed0;
-            const bool vec_res = res_vec && packed0 + 32 <= a.n;  // residuals by 16 bytes
             const uint32_t tsum = tlane + (uint32_t)(dd.s * C::kRows);
 #pragma unroll
             for (int c = 0; c < C::kAcc / 16; ++c)
@@ -571,11 +584,14 @@ cudaError_t launch_t(const LinearArgs &a, unsigned grid, cudaStream_t s) {
     return a.group == 32 ? launch_g<C, 4>(a, grid, s) : a.group == 64 ? launch_g<C, 2>(a, grid, s) : launch_g<C, 1>(a, grid, s);
 }
 
-// At most 14 warps of 144 registers per SM. Few rows: the weight stream asks
-// for converters; many: the sums ask for drains (80 rows a thread; 96 measured slower).
-using Small = Cfg<32, 4, 4, 2>;
-using Medium = Cfg<64, 8, 4, 1>;
-using Large = Cfg<160, 4, 8, 1>;
+// Few rows: the weight stream asks for two CTAs' converters and issuers per SM
+// (10 warps of 96 registers each; 32 rows x 4096 x 14336 gated 27 us against
+// 31.6 with two issuers a CTA, whose 80 registers spill, and 36 with one CTA).
+// Many: the sums ask for drains (64 rows a thread; 80 and 96 measured 5 % and
+// more slower at 8192 x 4096 x 4096 and ragged sizes).
+using Small = Cfg<32, 2, 4, 4, 1, 2>;
+using Medium = Cfg<64, 2, 8, 4, 2, 1>;
+using Large = Cfg<128, 2, 4, 8, 2, 1>;
 
 }  // namespace
 
