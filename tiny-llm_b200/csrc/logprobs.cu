@@ -6,15 +6,17 @@
 // One pass over a row: every thread keeps the maximum of its elements and,
 // relative to it, the two sums (fp32, base 2), rescaled when the maximum
 // grows, so the row is read from HBM once and nothing of it is kept; the
-// logits' bytes bound it. Rows too few to fill the machine are split over the
-// CTAs of a cluster, which join in distributed shared memory.
+// logits' bytes bound it, closely followed by the instructions an element
+// takes (a conversion, the exponential, and half each of four packed ones).
+// Rows too few to fill the machine are split over the CTAs of a cluster,
+// which join in distributed shared memory.
 //
-// The alternatives cost next to nothing in the pass: of the CTA's maxima over
-// groups of four threads the n-th largest is a lower bound of the n-th
-// largest logit, and only threads whose own maximum reaches it (about n of
-// them) can hold one of the n. Their elements are read again (from L2), the
-// ones that reach the bound are listed and ranked by counting. A list that
-// overflows (thousands of equal logits) is replaced by n searches of the
+// The alternatives cost next to nothing in the pass: of the maxima of 16 to
+// 128 groups of threads the n-th largest is a lower bound of the n-th largest
+// logit, and only threads whose own maximum reaches it can hold one of the n.
+// Their elements are looked at again (in registers where they fit, else from
+// L2), the ones that reach the bound are listed and ranked by counting. A list
+// that overflows (thousands of equal logits) is replaced by n searches of the
 // slice for the largest element behind the last one found.
 //
 // Sums are combined in a fixed order: a row's result does not depend on
@@ -36,7 +38,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kGroups = kThreads / 4;  // at least kMaxTop
+constexpr int kGroups = kThreads / 4;  // at most; at least kMaxTop
+constexpr int kU = 4;                  // vectors in flight per thread
 constexpr int kMaxTop = kLogprobMaxTop;
 constexpr int kCand = 1024;
 constexpr int kMaxCluster = 8;
@@ -69,6 +72,17 @@ struct Vec<__half> {
         return max_nan(__low2float(m), __high2float(m));
     }
     static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+    // Whether, relative to a maximum m, an element at the type's lowest value
+    // weighs nothing: then -inf may be taken for it, which keeps every z finite
+    // without a comparison in fp32 for each.
+    static __device__ __forceinline__ bool lowest_is_nothing(float m, float c) { return (m + 65504.f) * c > 160.f; }
+    static __device__ __forceinline__ uint4 raise(uint4 v) {
+        const __half2 low = __halves2half2(__ushort_as_half(0xFBFF), __ushort_as_half(0xFBFF));
+        __half2 *h = reinterpret_cast<__half2 *>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], low);
+        return v;
+    }
 };
 template <>
 struct Vec<__nv_bfloat16> {
@@ -87,6 +101,9 @@ struct Vec<__nv_bfloat16> {
         return max_nan(__low2float(m), __high2float(m));
     }
     static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+    // (z of the lowest value is not finite for every c: clamped one by one)
+    static __device__ __forceinline__ bool lowest_is_nothing(float, float) { return false; }
+    static __device__ __forceinline__ uint4 raise(uint4 v) { return v; }
 };
 template <>
 struct Vec<float> {
@@ -102,6 +119,9 @@ struct Vec<float> {
                        max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
     }
     static __device__ __forceinline__ float to_float(float v) { return v; }
+    // (z of the lowest value is not finite for every c: clamped one by one)
+    static __device__ __forceinline__ bool lowest_is_nothing(float, float) { return false; }
+    static __device__ __forceinline__ uint4 raise(uint4 v) { return v; }
 };
 
 // Sums of a set of elements relative to their maximum m: l = sum 2^z and
@@ -137,6 +157,20 @@ __device__ __forceinline__ void add(Sums &s, float x, float c) {
     s.t = fmaf(e, z, s.t);
 }
 
+// Two elements at a time, z by one packed FMA. nmc: -m c rounded once; what
+// that rounding shifts every z by is put right at the end (Sums are relative
+// to nmc / -c then, see unshift).
+struct Sums2 {
+    uint64_t l, t;
+};
+__device__ __forceinline__ void add2(Sums2 &s, float x0, float x1, uint64_t c2, uint64_t nmc2) {
+    float z0, z1;
+    ptx::f2_unpack(ptx::f2_fma(ptx::f2_pack(x0, x1), c2, nmc2), z0, z1);
+    const uint64_t e = ptx::f2_pack(ptx::ex2(z0), ptx::ex2(z1));
+    s.l = ptx::f2_add(s.l, e);
+    s.t = ptx::f2_fma(e, ptx::f2_pack(z0, z1), s.t);
+}
+
 struct Best {
     float v;
     int i;
@@ -154,6 +188,7 @@ struct Shared {
     Best list[kMaxTop];       // read by the cluster
     Best cand[kCand];         // candidates; then the cluster's lists
     Best red[kWarps];
+    int rank[kMaxCluster * kMaxTop];
 };
 static_assert(kMaxCluster * kMaxTop <= kCand, "the cluster's lists fit the candidates' place");
 
@@ -191,9 +226,9 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
         rebase(s, max_nan(fmaxf(v, -FLT_MAX), v), c);
         add(s, v, c);
     }
-    constexpr int kU = 4;  // vectors in flight per thread
+    const bool once = nvec <= kThreads * kU;  // one round: the elements stay in registers
+    uint4 v[kU];
     for (int i0 = tid; i0 < nvec; i0 += kThreads * kU) {
-        uint4 v[kU];
 #pragma unroll
         for (int u = 0; u < kU; ++u)
             if (i0 + u * kThreads < nvec) v[u] = __ldg(xv + i0 + u * kThreads);
@@ -205,14 +240,38 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
         // a batch of -inf alone moves the maximum to -FLT_MAX, not to -inf:
         // differences to it stay numbers
         rebase(s, max_nan(s.m, max_nan(m, -FLT_MAX)), c);
+        if (Vec<T>::lowest_is_nothing(s.m, c)) {
+            const float nmc = -s.m * c, shift = fmaf(s.m, c, nmc);  // z of the maximum itself: the rounding of nmc
+            const uint64_t c2 = ptx::f2_pack(c, c), nmc2 = ptx::f2_pack(nmc, nmc);
+            Sums2 p = {0ull, 0ull}, q = {0ull, 0ull};
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
-            if (i0 + u * kThreads < nvec) {
-                float f[N];
-                Vec<T>::load(v[u], f);
+            for (int u = 0; u < kU; ++u)
+                if (i0 + u * kThreads < nvec) {
+                    float f[N];
+                    Vec<T>::load(Vec<T>::raise(v[u]), f);
 #pragma unroll
-                for (int e = 0; e < N; ++e) add(s, f[e], c);
-            }
+                    for (int e = 0; e < N; e += 4) {
+                        add2(p, f[e], f[e + 1], c2, nmc2);
+                        add2(q, f[e + 2], f[e + 3], c2, nmc2);
+                    }
+                }
+            float l0, l1, t0, t1;
+            ptx::f2_unpack(ptx::f2_add(p.l, q.l), l0, l1);
+            ptx::f2_unpack(ptx::f2_add(p.t, q.t), t0, t1);
+            // every weight came out 2^shift times too large, every z by shift
+            const float l = l0 + l1, t = fmaf(-shift, l, t0 + t1), k = ptx::ex2(-shift);
+            s.l = fmaf(l, k, s.l);
+            s.t = fmaf(t, k, s.t);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+                if (i0 + u * kThreads < nvec) {
+                    float f[N];
+                    Vec<T>::load(v[u], f);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) add(s, f[e], c);
+                }
+        }
     }
 
     // ---- the CTA's sums, and the bound of its alternatives ----
@@ -224,22 +283,33 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
     }
     if (lane == 0) sh.sums[warp] = s;
     const int top = a.top;
+    // groups of 32, 16, 8 or 4 lanes: half as many again as alternatives, so
+    // that the bound is not far below the n-th largest
+    const int lanes = top <= 10 ? 32 : top <= 21 ? 16 : top <= 42 ? 8 : 4;
     if (top > 0) {
-        float g = max_nan(own, __shfl_xor_sync(0xffffffffu, own, 1));
-        g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, 2));
-        if ((lane & 3) == 0) sh.gmax[tid >> 2] = g;
+        float g = own;
+        for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if ((lane & (lanes - 1)) == 0) sh.gmax[tid / lanes] = g;
     }
     __syncthreads();
-    if (tid == 0) {
-        Sums t = sh.sums[0];
-        for (int w = 1; w < kWarps; ++w) t = join(t, sh.sums[w], c);
-        sh.cta = t;
+    if (warp == 0) {
+        Sums t = lane < kWarps ? sh.sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+        for (int o = kWarps / 2; o > 0; o >>= 1) {
+            const Sums b = {__shfl_down_sync(0xffffffffu, t.m, o), __shfl_down_sync(0xffffffffu, t.l, o),
+                            __shfl_down_sync(0xffffffffu, t.t, o)};
+            t = join(t, b, c);
+        }
+        if (lane == 0) sh.cta = t;
     }
     if (top > 0) {
-        if (tid < kGroups) {  // the group maximum of rank top - 1 (a NaN has rank 0: the row is answered with NaN)
-            const float g = sh.gmax[tid];
+        const int groups = kThreads / lanes;
+        const int at = tid - (kThreads - kGroups);  // the last warps: warp 0 joins the sums
+        if (at >= 0 && at < groups) {  // the group maximum of rank top - 1 (a NaN has rank 0: the row is answered with NaN)
+            const float g = sh.gmax[at];
             int r = 0;
-            for (int j = 0; j < kGroups; ++j) r += before(sh.gmax[j], j, g, tid);
+#pragma unroll 8
+            for (int j = 0; j < groups; ++j) r += before(sh.gmax[j], j, g, at);
             if (r == top - 1) sh.bound = g;
         }
         __syncthreads();
@@ -251,18 +321,34 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
             }
         };
         if (single >= 0) offer(Vec<T>::to_float(x[single]), single);
-        // the whole warp reads the elements of each of its threads that may hold one
-        unsigned todo = __ballot_sync(0xffffffffu, own >= bound && own > -INFINITY);
-        while (todo) {
-            const int from = (warp << 5) + __ffs(todo) - 1;
-            todo &= todo - 1;
-            for (int i = from + lane * kThreads; i < nvec; i += 32 * kThreads) {
-                float f[N];
-                const uint4 v = __ldg(xv + i);
-                if (Vec<T>::max(v) >= bound) {
-                    Vec<T>::load(v, f);
+        const bool mine = own >= bound && own > -INFINITY;
+        if (once) {
+            if (mine) {
 #pragma unroll
-                    for (int e = 0; e < N; ++e) offer(f[e], lo + head + i * N + e);
+                for (int u = 0; u < kU; ++u) {
+                    const int i = tid + u * kThreads;
+                    if (i < nvec && Vec<T>::max(v[u]) >= bound) {
+                        float f[N];
+                        Vec<T>::load(v[u], f);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) offer(f[e], lo + head + i * N + e);
+                    }
+                }
+            }
+        } else {
+            // the whole warp reads the elements of each of its threads that may hold one
+            unsigned todo = __ballot_sync(0xffffffffu, mine);
+            while (todo) {
+                const int from = (warp << 5) + __ffs(todo) - 1;
+                todo &= todo - 1;
+                for (int i = from + lane * kThreads; i < nvec; i += 32 * kThreads) {
+                    float f[N];
+                    const uint4 w = __ldg(xv + i);
+                    if (Vec<T>::max(w) >= bound) {
+                        Vec<T>::load(w, f);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) offer(f[e], lo + head + i * N + e);
+                    }
                 }
             }
         }
@@ -315,25 +401,43 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
     if (split > 1) {
         cluster.sync();
         if (rank == 0) {
-            for (int q = 1; q < split; ++q) all = join(all, *cluster.map_shared_rank(&sh.cta, q), c);
+            // lane q has CTA q's sums; joined in a fixed order
+            Sums t = lane < split ? *cluster.map_shared_rank(&sh.cta, lane) : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll
+            for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
+                const Sums b = {__shfl_down_sync(0xffffffffu, t.m, o), __shfl_down_sync(0xffffffffu, t.l, o),
+                                __shfl_down_sync(0xffffffffu, t.t, o)};
+                t = join(t, b, c);
+            }
+            all = {__shfl_sync(0xffffffffu, t.m, 0), __shfl_sync(0xffffffffu, t.l, 0), __shfl_sync(0xffffffffu, t.t, 0)};
             if (top > 0) {
-                // every list in its place of `cand`, missing entries last
+                // every list in its place of `cand`, missing entries last; an
+                // entry's rank is its own place and those before it in the
+                // other lists, which are sorted
+                int f = lane < split ? cluster.map_shared_rank(&sh, lane)->found : 0;
                 for (int j = tid; j < split * top; j += kThreads) {
                     const int q = j / top, n = j % top;
                     const Shared *o = cluster.map_shared_rank(&sh, q);
                     sh.cand[j] = n < o->found ? o->list[n] : Best{-INFINITY, 0x7fffffff};
+                    sh.rank[j] = n;
+                }
+#pragma unroll
+                for (int o = kMaxCluster / 2; o > 0; o >>= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
+                found = min(__shfl_sync(0xffffffffu, f, 0), top);
+                __syncthreads();
+                for (int j = tid; j < split * top * split; j += kThreads) {
+                    const int e = j / split, q = j % split;
+                    const Best b = sh.cand[e];
+                    if (q == e / top || b.i == 0x7fffffff) continue;
+                    const Best *l = sh.cand + q * top;
+                    int n = 0;
+                    for (int step = kMaxTop; step > 0; step >>= 1)
+                        if (n + step <= top && before(l[n + step - 1].v, l[n + step - 1].i, b.v, b.i)) n += step;
+                    if (n > 0) atomicAdd(&sh.rank[e], n);
                 }
                 __syncthreads();
-                for (int j = tid; j < split * top; j += kThreads) {
-                    const Best b = sh.cand[j];
-                    if (b.i == 0x7fffffff) continue;
-                    int r = 0;
-                    for (int q = 0; q < split * top; ++q) r += before(sh.cand[q].v, sh.cand[q].i, b.v, b.i);
-                    if (r < top) sh.list[r] = b;
-                }
-                found = 0;
-                for (int q = 0; q < split; ++q) found += cluster.map_shared_rank(&sh, q)->found;
-                found = min(found, top);
+                for (int j = tid; j < split * top; j += kThreads)
+                    if (sh.cand[j].i != 0x7fffffff && sh.rank[j] < top) sh.list[sh.rank[j]] = sh.cand[j];
                 __syncthreads();
             }
         }
