@@ -55,6 +55,7 @@ constexpr int kStepK = lin::kBlockK;  // rows of K per ring stage
 constexpr int kACols = kStepK / 2;  // TMEM columns of one (fp16 pairs along K)
 constexpr int kRaw = 2 * 2 * lin::kHalfBytes;  // packed weights of a step
 constexpr int kMaxStages = 8;
+constexpr int kMaxSplit = 8;       // CTAs of a cluster that share K
 constexpr int kOutRows = 16;       // rows a drain warp writes at a time
 constexpr int kOutPitch = 36;      // floats of such a row: 32 columns, padded to 16 bytes and other banks
 constexpr long long kWait = 4000000000ll;  // cycles: about 2 s
@@ -192,6 +193,39 @@ __device__ __forceinline__ void write_rows_act(const LinearArgs &a, const float 
     case 3: return write_rows<3, GATED>(a, st, lane, row0, nrows, packed0, have_res, q0, q1);
     case 4: return write_rows<4, GATED>(a, st, lane, row0, nrows, packed0, have_res, q0, q1);
     default: return write_rows<0, GATED>(a, st, lane, row0, nrows, packed0, have_res, q0, q1);
+    }
+}
+
+// Four outputs of a row from their sums (v, and u of a gated pair).
+template <int ACT>
+__device__ __forceinline__ void finish4(const LinearArgs &a, const float (&v)[4], const float (&u)[4], long long row,
+                                        long long n0) {
+    const int valid = (int)min(4ll, a.n - n0);
+    const __half *bias = static_cast<const __half *>(a.bias), *bias2 = static_cast<const __half *>(a.bias2);
+    const __half *res = a.residual ? static_cast<const __half *>(a.residual) + row * a.residual_stride + n0 : nullptr;
+    __half *y = static_cast<__half *>(a.y) + row * a.y_stride + n0;
+    uint32_t o[2];
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int at = min(j + e, valid - 1);  // (outputs past the last column are not written)
+            float x = v[j + e];
+            if (bias) x += __half2float(bias[n0 + at]);
+            x = lin::activate(ACT, x);
+            if (a.gated) x *= u[j + e] + (bias2 ? __half2float(bias2[n0 + at]) : 0.f);
+            else if (res) x += __half2float(res[at]);
+            f[e] = x;
+        }
+        o[j / 2] = ptx::pack_half2(f[0], f[1]);
+    }
+    if (valid == 4 && (reinterpret_cast<uintptr_t>(y) & 7) == 0) {
+        *reinterpret_cast<uint2 *>(y) = make_uint2(o[0], o[1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < valid) y[j] = __ushort_as_half((unsigned short)(o[j / 2] >> (16 * (j & 1))));
     }
 }
 
@@ -518,29 +552,39 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         cluster.sync();
         const TilePos p = tile_pos(first, ntiles, nrt);
         const float *part = reinterpret_cast<const float *>(smem);
-        const int oc = a.gated ? kM / 2 : kM, nrows = min(RT, a.rows - p.rt * RT);
-        const __half *bias = static_cast<const __half *>(a.bias), *bias2 = static_cast<const __half *>(a.bias2);
+        const int nrows = min(RT, a.rows - p.rt * RT), chunks = a.gated ? kM / 8 : kM / 4;  // fours of outputs
         ptx::griddep_wait();
-        for (int i = rank * C::kThreads + threadIdx.x; i < nrows * oc; i += csplit * C::kThreads) {
-            const int r = i / oc, c = i % oc;
-            const long long n = (long long)p.nt * oc + c, row = (long long)p.rt * RT + r;
-            if (n >= a.n) continue;
-            const int c0 = a.gated ? (c >> 3) * 16 + (c & 7) : c;
-            float v = 0.f, u = 0.f;
-            for (int k = 0; k < csplit; ++k) {
-                const float *o = cluster.map_shared_rank(part + r * kM + c0, k);
-                v += o[0];
-                if (a.gated) u += o[8];
+        // every CTA's four sums asked for at once, added in rank order
+        auto total4 = [&](const float *mine, float (&t)[4]) {
+            float4 x[kMaxSplit];
+#pragma unroll
+            for (int k = 0; k < kMaxSplit; ++k)
+                if (k < csplit) x[k] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(mine, k));
+            t[0] = t[1] = t[2] = t[3] = 0.f;
+#pragma unroll
+            for (int k = 0; k < kMaxSplit; ++k)
+                if (k < csplit) {
+                    t[0] += x[k].x;
+                    t[1] += x[k].y;
+                    t[2] += x[k].z;
+                    t[3] += x[k].w;
+                }
+        };
+        for (int i = rank * C::kThreads + threadIdx.x; i < nrows * chunks; i += csplit * C::kThreads) {
+            const int r = i / chunks, c = i % chunks;
+            const long long n0 = ((long long)p.nt * chunks + c) * 4, row = (long long)p.rt * RT + r;
+            if (n0 >= a.n) continue;
+            const float *mine = part + r * kM + (a.gated ? (c >> 1) * 16 + (c & 1) * 4 : 4 * c);
+            float v[4], u[4] = {0.f, 0.f, 0.f, 0.f};
+            total4(mine, v);
+            if (a.gated) total4(mine + 8, u);
+            switch (a.act) {
+            case 1: finish4<1>(a, v, u, row, n0); break;
+            case 2: finish4<2>(a, v, u, row, n0); break;
+            case 3: finish4<3>(a, v, u, row, n0); break;
+            case 4: finish4<4>(a, v, u, row, n0); break;
+            default: finish4<0>(a, v, u, row, n0);
             }
-            if (bias) v += __half2float(bias[n]);
-            v = lin::activate(a.act, v);
-            if (a.gated) {
-                if (bias2) u += __half2float(bias2[n]);
-                v *= u;
-            } else if (a.residual) {
-                v += __half2float(static_cast<const __half *>(a.residual)[row * a.residual_stride + n]);
-            }
-            static_cast<__half *>(a.y)[row * a.y_stride + n] = __float2half_rn(v);
         }
         __syncwarp();
         cluster.sync();  // no CTA leaves while another may still read its shared memory
@@ -604,7 +648,7 @@ cudaError_t launch_linear_tc(LinearArgs a, int num_sms, cudaStream_t s) {
     const long long slots = (long long)num_sms * (small ? Small::kPerSm : Large::kPerSm);
     const int nblocks = lin::blocks(a.k);
     a.csplit = 1;
-    while (a.csplit < 8 && total * a.csplit * 2 <= slots && nblocks / (a.csplit * 2) >= 4) a.csplit *= 2;
+    while (a.csplit < kMaxSplit && total * a.csplit * 2 <= slots && nblocks / (a.csplit * 2) >= 4) a.csplit *= 2;
     const unsigned grid = (unsigned)(a.csplit > 1 ? total * a.csplit : std::min<long long>(total, slots));
     return small ? launch_t<Small>(a, grid, s)
            : a.row_tile <= Medium::kRows ? launch_t<Medium>(a, grid, s)

@@ -36,14 +36,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kGroups = kThreads / 4;  // at most; at least kMaxTop
-constexpr int kU = 4;                  // vectors in flight per thread
 constexpr int kMaxTop = kLogprobMaxTop;
 constexpr int kCand = 1024;
 constexpr int kMaxCluster = 8;
-static_assert(kGroups >= kMaxTop, "the bound needs as many groups as alternatives");
+constexpr int kMaxWarps = 16;
+constexpr int kMaxGroups = 128;        // of threads, for the bound; at least kMaxTop
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -179,23 +176,28 @@ struct Best {
 __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
 struct Shared {
-    Sums sums[kWarps];
+    Sums sums[kMaxWarps];
     Sums cta;                 // read by the cluster
-    float gmax[kGroups];
+    float gmax[kMaxGroups];
     float bound;
     int count;
     int found;                // entries of list
     Best list[kMaxTop];       // read by the cluster
     Best cand[kCand];         // candidates; then the cluster's lists
-    Best red[kWarps];
+    Best red[kMaxWarps];
     int rank[kMaxCluster * kMaxTop];
 };
 static_assert(kMaxCluster * kMaxTop <= kCand, "the cluster's lists fit the candidates' place");
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
-    constexpr int N = Vec<T>::kN;
+// kThreads: 512 where few CTAs share the device, 256 (four CTAs an SM) where
+// the end of one row has to hide behind the passes of others.
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+    constexpr int N = Vec<T>::kN, kWarps = kThreads / 32;
+    constexpr int kU = kThreads == 256 ? 8 : 4;  // vectors in flight per thread
     __shared__ Shared sh;
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = a.split, rank = blockIdx.x % split;
     const int row = blockIdx.x / split;
@@ -283,9 +285,10 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
     }
     if (lane == 0) sh.sums[warp] = s;
     const int top = a.top;
-    // groups of 32, 16, 8 or 4 lanes: half as many again as alternatives, so
+    // groups of 32, 16, 8, 4 or 2 lanes: half as many again as alternatives, so
     // that the bound is not far below the n-th largest
-    const int lanes = top <= 10 ? 32 : top <= 21 ? 16 : top <= 42 ? 8 : 4;
+    int lanes = 32;
+    while (kThreads / lanes < top + top / 2) lanes >>= 1;
     if (top > 0) {
         float g = own;
         for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
     }
     if (top > 0) {
         const int groups = kThreads / lanes;
-        const int at = tid - (kThreads - kGroups);  // the last warps: warp 0 joins the sums
+        const int at = tid - (kThreads - kMaxGroups);  // the last warps: warp 0 joins the sums
         if (at >= 0 && at < groups) {  // the group maximum of rank top - 1 (a NaN has rank 0: the row is answered with NaN)
             const float g = sh.gmax[at];
             int r = 0;
@@ -471,36 +474,44 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(const __grid_cons
     if (split > 1) cluster.sync();  // no CTA leaves while rank 0 may still read its shared memory
 }
 
-template <typename T>
-cudaError_t launch_t(const LogprobArgs &a, cudaStream_t s) {
+template <typename T, int kThreads>
+cudaError_t launch_n(const LogprobArgs &a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows * (unsigned)a.split);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)a.split;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a);
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, kThreads>, a);
+}
+
+template <typename T>
+cudaError_t launch_t(const LogprobArgs &a, int num_sms, cudaStream_t s) {
+    return (long long)a.rows * a.split > 2ll * num_sms ? launch_n<T, 256>(a, s) : launch_n<T, 512>(a, s);
 }
 
 }  // namespace
 
 cudaError_t launch_logprobs(LogprobArgs a, int dtype, int num_sms, cudaStream_t s) {
     if (a.rows <= 0) return cudaSuccess;
-    // Rows split over a cluster until they fill the SMs' CTA slots, as long as
-    // a thread keeps a few vectors.
+    // Rows split over a cluster until there is a CTA for every SM or two, as
+    // long as a thread keeps two vectors (with twice as many CTAs 64 rows of
+    // 128256 take 17.5 us instead of 14.8).
     const int per = dtype == 2 ? 4 : 8;
     a.split = 1;
-    while (a.split < kMaxCluster && (long long)a.rows * a.split * 2 <= 2ll * num_sms &&
-           a.vocab / (a.split * 2) >= 2 * per * kThreads)
+    while (a.split < kMaxCluster && (long long)a.rows * a.split <= num_sms &&
+           a.vocab / (a.split * 2) >= 2 * per * 512)
         a.split *= 2;
     switch (dtype) {
-    case 0: return launch_t<__half>(a, s);
-    case 1: return launch_t<__nv_bfloat16>(a, s);
-    case 2: return launch_t<float>(a, s);
+    case 0: return launch_t<__half>(a, num_sms, s);
+    case 1: return launch_t<__nv_bfloat16>(a, num_sms, s);
+    case 2: return launch_t<float>(a, num_sms, s);
     default: return cudaErrorInvalidValue;
     }
 }
