@@ -308,3 +308,92 @@ def test_a_layers_end_and_the_head():
     assert ((lp.double() - logp.max(1).values).abs() < 4e-6).all()
     assert ((ent.double() + (logp.exp() * logp).sum(1)).abs() < 4e-5).all()
     assert np.isfinite(h.float().cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("rows", [3, 40, 130])
+@pytest.mark.parametrize("gated", [False, True])
+def test_unaligned_outputs_and_epilogue_inputs(rows, gated):
+    """y, bias and residual on odd elements (2-byte aligned only)."""
+    import torch
+    k, n, group = 320, 136, 64
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    A, B = Weight(k, n, group, gen), Weight(k, n, group, gen)
+    packed = pack(k, n, group, A, B if gated else None)
+    x = make_x(rows, k, gen)
+    bias = torch.randn(2, n + 1, device="cuda", generator=gen).half()
+    res = torch.randn(rows * (n + 8) + 1, device="cuda", generator=gen).half()
+    y = torch.full((rows * (n + 8) + 2,), 7.0, device="cuda", dtype=torch.float16)
+    even = torch.empty(rows, n, device="cuda", dtype=torch.float16)  # the same with everything aligned
+    b0, b1, r0 = bias[0, 1:].clone(), bias[1, 1:].clone(), res[1:].view(rows, n + 8)[:, :n].clone()
+    if gated:
+        T.linear_gated(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y[1:].data_ptr(), activation=4,
+                       bias=bias[0, 1:].data_ptr(), bias_up=bias[1, 1:].data_ptr(), y_stride=n + 8)
+        T.linear_gated(x.data_ptr(), rows, packed.data_ptr(), k, n, group, even.data_ptr(), activation=4,
+                       bias=b0.data_ptr(), bias_up=b1.data_ptr())
+    else:
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y[1:].data_ptr(), activation=2,
+                 bias=bias[0, 1:].data_ptr(), residual=res[1:].data_ptr(), y_stride=n + 8, residual_stride=n + 8)
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, even.data_ptr(), activation=2,
+                 bias=b0.data_ptr(), residual=r0.data_ptr())
+    torch.cuda.synchronize()
+    got = y[1:-1].view(rows, n + 8)
+    assert torch.equal(got[:, :n], even) and (got[:, n:] == 7.0).all() and y[0] == 7.0 and y[-1] == 7.0
+
+
+@pytest.mark.parametrize("rows", [8, 20, 129])
+def test_far_rows(rows):
+    """Row offsets past 2^31 elements in the activations, residual and output."""
+    import torch
+    k, n, group = 136, 72, 128
+    stride = ((1 << 31) // (rows - 1) // 8 + 8) * 8
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    W = Weight(k, n, group, gen)
+    packed = pack(k, n, group, W)
+    buf = torch.empty(rows * stride, device="cuda", dtype=torch.float16)
+    far = buf.view(rows, stride)
+    x = make_x(rows, k, gen)
+    res = torch.randn(rows, n, device="cuda", generator=gen).half()
+    far[:, :k], far[:, 256:256 + n], far[:, 512:512 + n] = x, res, 7.0
+    y = torch.empty(rows, n, device="cuda", dtype=torch.float16)
+    T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr(), residual=res.data_ptr())
+    T.linear(far.data_ptr(), rows, packed.data_ptr(), k, n, group, far[:, 512:].data_ptr(), residual=far[:, 256:].data_ptr(),
+             x_stride=stride, y_stride=stride, residual_stride=stride)
+    torch.cuda.synchronize()
+    assert torch.equal(far[:, 512:512 + n], y)
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls of every kernel are captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    script = """
+import sys, torch
+sys.path[:0] = sys.argv[1:]
+import tiny_llm_b200 as T
+k, n = 512, 192
+w = torch.randint(-128, 128, (k, n), device="cuda", dtype=torch.int16).to(torch.int8)
+s = torch.rand(4, n, device="cuda").half()
+p = torch.empty(T.linear_packed_bytes(k, n, 128), device="cuda", dtype=torch.uint8)
+T.pack_linear_weight(w.data_ptr(), s.data_ptr(), k, n, 128, p.data_ptr())
+x = torch.randn(300, k, device="cuda").half()
+y = torch.zeros(5, 300, n, device="cuda", dtype=torch.float16)
+lp = torch.zeros(2, 300, device="cuda")
+t = torch.zeros(300, device="cuda", dtype=torch.int32)
+torch.cuda.synchronize()
+def calls(out, lps, stream):
+    for i, rows in enumerate((3, 20, 50, 300)):
+        T.linear(x.data_ptr(), rows, p.data_ptr(), k, n, 128, out[i].data_ptr(), stream=stream)
+    T.token_logprobs(out[3].data_ptr(), 300, n, t.data_ptr(), lps.data_ptr(), stream=stream)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    calls(y, lp[0], torch.cuda.current_stream().cuda_stream)
+g.replay()
+torch.cuda.synchronize()
+z = torch.zeros_like(y)
+calls(z, lp[1], 0)
+torch.cuda.synchronize()
+assert torch.equal(y, z) and torch.equal(lp[0], lp[1]) and y[:4].abs().amax((1, 2)).min() > 0
+"""
+    root = Path(T.__file__).resolve().parents[1]
+    subprocess.run([sys.executable, "-c", script, str(root)], check=True, timeout=300)

@@ -249,7 +249,8 @@ struct LinearArgs {
     int csplit;               // CTAs of a cluster that share K (set by the launcher)
     int row_tile;             // rows of a tile (set by launch_linear_tc)
 };
-cudaError_t launch_linear(LinearArgs a, int num_sms, cudaStream_t s);     // few rows: linear.cu
+constexpr int kLinearFewRows = 8;
+cudaError_t launch_linear(LinearArgs a, int num_sms, cudaStream_t s);     // up to kLinearFewRows rows: linear.cu
 cudaError_t launch_linear_tc(LinearArgs a, int num_sms, cudaStream_t s);  // more: linear_tc.cu
 // w2/s2: the other projection of a gated pair, or nullptr.
 cudaError_t launch_linear_pack(const int8_t *w, const void *s, const int8_t *w2, const void *s2, int k, int n, int group,

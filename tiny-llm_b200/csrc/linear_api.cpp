@@ -16,8 +16,6 @@ namespace {
 
 constexpr int kMaxRows = 1 << 20, kMaxK = 1 << 20, kMaxN = 1 << 22;
 
-constexpr int kFewRows = 8;
-
 bool misaligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
 // TL_OK, or the refusal of a weight's shape.
@@ -53,7 +51,8 @@ int linear(const char *ctx, tllm::LinearArgs a, cudaStream_t stream) {
         return set_thread_error(TL_ERR_INVALID_ARG, "%s: the strides of output and residual must be at least n", ctx);
     const int sms = tllm::current_device_sms();
     if (sms == 0) return set_thread_error(TL_ERR_NO_DEVICE, "%s: no CUDA device", ctx);
-    const cudaError_t e = a.rows <= kFewRows ? tllm::launch_linear(a, sms, stream) : tllm::launch_linear_tc(a, sms, stream);
+    const cudaError_t e = a.rows <= tllm::kLinearFewRows ? tllm::launch_linear(a, sms, stream)
+                                                         : tllm::launch_linear_tc(a, sms, stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_thread_error(TL_ERR_CUDA, "%s: launch failed: %s", ctx, cudaGetErrorString(e));
