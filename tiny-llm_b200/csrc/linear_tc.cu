@@ -14,15 +14,16 @@
 //   converters  thread = weight column: 64 bytes from shared memory, to 64
 //               fp16, one tcgen05.st of 32 columns: the K-major A operand of
 //               half a step (four warps do both halves, eight one each);
-//   MMA         one thread each of two warps: eight UMMAs (K = 16) per step, A
+//   MMA         one thread each of one or two warps: eight UMMAs (K = 16) per step, A
 //               in TMEM, B in shared memory; the scale groups take two
-//               accumulators in turn, each with an issuing warp of its own;
+//               accumulators in turn, with two warps each its own;
 //   drains      thread = weight column (TMEM lane): when a group is complete,
 //               acc += scale * sum for the thread's rows, in registers; after
 //               the last group the epilogue from them.
-// So the tensor cores never wait for the scaling (the other accumulator is
-// filled meanwhile), and the CTAs are persistent: the next tile's first
-// groups run while a tile's outputs are written.
+// So one accumulator is filled while the other is scaled, and the CTAs are
+// persistent: the next tile's first groups run while a tile's outputs are
+// written. The chain conversion - UMMAs - drain sets the pace, not the tensor
+// pipe (39 % active at 1024 x 4096 x 14336 gated).
 //
 // A wait that succeeds at once costs an issuing thread about 110 cycles, a
 // commit 80, a UMMA 75 or its pipe time (rows / 2) while the pipe's queue is
@@ -64,9 +65,9 @@ struct alignas(64) Map {  // a tensor map, opaque here
     unsigned char bytes[128];
 };
 
-// kRows: most rows of a tile. kNA: A operand stages in TMEM. kCW, kDW: converter and drain warps (sets of
-// four, one per TMEM lane quarter). kIssue: warps that issue UMMAs. kPerSm:
-// CTAs per SM.
+// kRows: most rows of a tile. kNA: A operand stages in TMEM. kCW, kDW:
+// converter and drain warps (sets of four, one per TMEM lane quarter). kIssue:
+// warps that issue UMMAs. kPerSm: CTAs per SM.
 template <int kRows_, int kNA_, int kCW_, int kDW_, int kIssue_, int kPerSm_>
 struct Cfg {
     static constexpr int kNA = kNA_;
@@ -77,7 +78,7 @@ struct Cfg {
     static constexpr int kThreads = 32 * (kDW + kCW + 1 + kIssue);
     static constexpr int kAcc = kRows / kDrainSets;  // rows per drain thread
     static constexpr uint32_t kTmemCols = 2 * kRows + kNA * kACols <= 256 ? 256 : 512;
-    static constexpr int kRing = (kPerSm == 2 ? 96 : kDW > 12 ? 176 : 192) * 1024;
+    static constexpr int kRing = (kPerSm == 2 ? 96 : 192) * 1024;
     static constexpr int kOut = kDW * kOutRows * kOutPitch * 4;  // the drain warps' rows on their way out
     static constexpr int kBars = (2 * kMaxStages + kNA + 5) * 8;
     static constexpr int kSmem = 1024 + kRing + kOut + kBars + 16;
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kRing + C::kOut);
     const uint32_t full_u = ptx::smem_u32(bars);           // [stages] weights and activations landed
     const uint32_t empty_u = full_u + 8 * kMaxStages;      // [stages] multiplied: the stage and its A operand are free
-    const uint32_t afull_u = empty_u + 8 * kMaxStages;     // [C::kNA] A operand in TMEM
+    const uint32_t afull_u = empty_u + 8 * kMaxStages;     // [kNA] A operand in TMEM
     const uint32_t dfull_u = afull_u + 8 * C::kNA;            // [2] a group's sums complete
     const uint32_t dempty_u = dfull_u + 16;                // [2] ... and drained
     const uint32_t done_u = dempty_u + 16;                 // every UMMA complete
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     const int steps = b1 - b0;
     const int first = blockIdx.x / csplit, stride = gridDim.x / csplit;
     const int xhalf = RT * 128, stage_bytes = 2 * xhalf + kRaw;
-    const int NS = min(kMaxStages, C::kRing / stage_bytes);  // > C::kNA: a converter meets every phase it waits for
+    const int NS = min(kMaxStages, C::kRing / stage_bytes);  // > kNA: a converter meets every phase it waits for
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMaxStages; ++s) {

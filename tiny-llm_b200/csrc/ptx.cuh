@@ -49,19 +49,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
-// The same without blocking: whether the phase is complete now.
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 // ---- tcgen05 (5th-generation tensor cores, TMEM accumulators) ----------
 // TMEM allocation of `ncols` columns (a power of two >= 32) by one whole
 // warp; the base address is written to shared memory at dst.
@@ -181,9 +168,7 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
     }
 }
 
-// The same, bounded in SM clock cycles: reading the clock takes a few cycles
-// where %globaltimer takes about a microsecond, which a pipeline whose stages
-// wait for one another pays at every wait that does not succeed at once.
+// The same, bounded in SM clock cycles.
 __device__ __forceinline__ bool mbar_wait_cycles(uint32_t bar, uint32_t parity, long long limit) {
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
