@@ -397,3 +397,51 @@ assert torch.equal(y, z) and torch.equal(lp[0], lp[1]) and y[:4].abs().amax((1, 
 """
     root = Path(T.__file__).resolve().parents[1]
     subprocess.run([sys.executable, "-c", script, str(root)], check=True, timeout=300)
+
+
+@pytest.mark.parametrize("rows", [4, 33, 130])
+def test_logits_written_between_two_readers(rows):
+    """log probabilities -> product into the same logits -> log probabilities,
+    back to back and replayed: every reader sees the product before it, not
+    what an earlier reader loaded."""
+    import torch
+    k, vocab, group, top, n = 512, 4096, 128, 4, 24
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    W = Weight(k, vocab, group, gen)
+    packed = pack(k, vocab, group, W)
+    xs = [make_x(rows, k, gen) for _ in range(3)]
+    tokens = torch.arange(rows, device="cuda", dtype=torch.int32) * 7 % vocab
+    logits = torch.empty(rows, vocab, device="cuda", dtype=torch.float16)
+
+    def outputs(m):
+        return (torch.empty(m, rows, device="cuda"), torch.empty(m, rows, device="cuda"),
+                torch.empty(m, rows, top, device="cuda", dtype=torch.int32),
+                torch.empty(m, rows, top, device="cuda"))
+
+    def step(x, out, i, stream):
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, vocab, group, logits.data_ptr(), stream=stream)
+        T.token_logprobs(logits.data_ptr(), rows, vocab, tokens.data_ptr(), out[0][i].data_ptr(), out[1][i].data_ptr(),
+                         top, out[2][i].data_ptr(), out[3][i].data_ptr(), stream=stream)
+
+    ref, got = outputs(3), outputs(n)
+    for i, x in enumerate(xs):
+        step(x, ref, i, 0)
+        torch.cuda.synchronize()
+    assert not torch.equal(ref[0][0], ref[0][1])
+    stream = torch.cuda.Stream()
+    for i in range(n):
+        step(xs[i % 3], got, i, stream.cuda_stream)
+    torch.cuda.synchronize()
+    for g, r in zip(got, ref):
+        assert all(torch.equal(g[i], r[i % 3]) for i in range(n))
+    for g in got:
+        g.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(n):
+            step(xs[i % 3], got, i, torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for g, r in zip(got, ref):
+        assert all(torch.equal(g[i], r[i % 3]) for i in range(n))

@@ -86,10 +86,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         s_failed = 0;
     }
     __syncthreads();
-    // Programmatic dependent launch: the next kernel's CTAs may come as ours
-    // leave. Until the kernel before has completed they only ask L2 for their
-    // first weights (a prefetch: a later write of them still wins) and sleep.
-    ptx::griddep_launch_dependents();
+    // Programmatic dependent launch: until the kernel before has completed, only
+    // a prefetch of the first weights to L2 (a later write of them still wins).
+    // The next kernel is let in after the wait, so that nothing older than this
+    // kernel runs beside it; its CTAs come as ours leave.
     const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)tile * nblocks + b0) * unit;
     if (warp == kConsumers && lane == 0) {
         ptx::prefetch_tensormap(&xmap);
@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncwarp();
     ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
 
     if (warp == kConsumers) {
         // ---- producer (one lane) ----

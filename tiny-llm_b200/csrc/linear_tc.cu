@@ -279,6 +279,22 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     ptx::tc_fence_after_sync();
     const uint32_t tbase = s_tmem;             // accumulators at 0 and kRows, then the A stages
     const uint32_t acol = 2 * C::kRows;
+    // Programmatic dependent launch: until the kernel before has completed, only
+    // a prefetch of the first weights to L2 (a later write of them still wins).
+    // The next kernel is let in after the wait, so that nothing older than this
+    // kernel runs beside it.
+    if (warp == C::kProd && lane == 0) {
+        ptx::prefetch_tensormap(&xmap);
+        if (first < total) {
+            const TilePos p = tile_pos(first, ntiles, nrt);
+            const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)(2 * p.nt) * nblocks + b0) * unit;
+            const uint32_t bytes = (uint32_t)(min(NS, steps) * unit);
+            ptx::bulk_prefetch_l2(w, bytes);
+            if (2 * p.nt + 1 < tiles64) ptx::bulk_prefetch_l2(w + (long long)nblocks * unit, bytes);
+        }
+    }
+    __syncwarp();
+    ptx::griddep_wait();
     ptx::griddep_launch_dependents();
 
     // (A wait for "empty" starts on the parity of the round before: a fresh
@@ -286,18 +302,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     if (warp == C::kProd) {
         if (lane == 0) {
             // ---- producer ----
-            // Programmatic dependent launch: until the kernel before has
-            // completed, only a prefetch of the first weights to L2 (a later
-            // write of them still wins).
-            ptx::prefetch_tensormap(&xmap);
-            if (first < total) {
-                const TilePos p = tile_pos(first, ntiles, nrt);
-                const uint8_t *w = static_cast<const uint8_t *>(a.packed) + ((long long)(2 * p.nt) * nblocks + b0) * unit;
-                const uint32_t bytes = (uint32_t)(min(NS, steps) * unit);
-                ptx::bulk_prefetch_l2(w, bytes);
-                if (2 * p.nt + 1 < tiles64) ptx::bulk_prefetch_l2(w + (long long)nblocks * unit, bytes);
-            }
-            ptx::griddep_wait();
             const uint64_t keep = ptx::l2_policy_evict_last();
             const uint64_t wpol = nrt > 1 ? keep : ptx::l2_policy_evict_first();  // weights: read once per row tile
             const uint8_t *packed = static_cast<const uint8_t *>(a.packed);
@@ -427,7 +431,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         float *st = out_rows + warp * kOutRows * kOutPitch;
         Ring dd;
         bool ok = true;
-        ptx::griddep_wait();
         for (int t = first; t < total; t += stride) {
             const TilePos p = tile_pos(t, ntiles, nrt);
             const int t64 = 2 * p.nt + (q >> 1);
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                                 (col & 63) * 2;
             int sub = 0;
             auto next_scale = [&]() -> unsigned short {  // converted where it is used, a group after it was asked for
-                const unsigned short v = __ldg(reinterpret_cast<const unsigned short *>(sp));
+                const unsigned short v = __ldcg(reinterpret_cast<const unsigned short *>(sp));
                 if (GPS == 1 || ++sub == GPS) {
                     sub = 0;
                     sp += unit - (GPS - 1) * (lin::kTileN * 2);
@@ -554,7 +557,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         const TilePos p = tile_pos(first, ntiles, nrt);
         const float *part = reinterpret_cast<const float *>(smem);
         const int nrows = min(RT, a.rows - p.rt * RT), chunks = a.gated ? kM / 8 : kM / 4;  // fours of outputs
-        ptx::griddep_wait();
         // every CTA's four sums asked for at once, added in rank order
         auto total4 = [&](const float *mine, float (&t)[4]) {
             float4 x[kMaxSplit];

@@ -196,8 +196,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     constexpr int N = Vec<T>::kN, kWarps = kThreads / 32;
     constexpr int kU = kThreads == 256 ? 8 : 4;  // vectors in flight per thread
     __shared__ Shared sh;
-    ptx::griddep_launch_dependents();
+    // Programmatic dependent launch: the kernel before may have written the
+    // logits while this one was already started, so they are read by coherent
+    // loads (ld.global.nc is for what no one writes in a kernel's lifetime),
+    // and the next kernel is let in only after the wait: nothing older than
+    // this kernel runs beside it.
     ptx::griddep_wait();
+    ptx::griddep_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = a.split, rank = blockIdx.x % split;
     const int row = blockIdx.x / split;
@@ -233,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     for (int i0 = tid; i0 < nvec; i0 += kThreads * kU) {
 #pragma unroll
         for (int u = 0; u < kU; ++u)
-            if (i0 + u * kThreads < nvec) v[u] = __ldg(xv + i0 + u * kThreads);
+            if (i0 + u * kThreads < nvec) v[u] = __ldcg(xv + i0 + u * kThreads);
         float m = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kU; ++u)
@@ -346,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
                 todo &= todo - 1;
                 for (int i = from + lane * kThreads; i < nvec; i += 32 * kThreads) {
                     float f[N];
-                    const uint4 w = __ldg(xv + i);
+                    const uint4 w = __ldcg(xv + i);
                     if (Vec<T>::max(w) >= bound) {
                         Vec<T>::load(w, f);
 #pragma unroll
