@@ -312,8 +312,8 @@ int tl_linear_pack(const int8_t *w, const void *scales, const int8_t *w_up, cons
 /* y[r][c] = act(sum_i x[r][i] w[i][c] scale[i / group_size][c] + bias[c]) + residual[r][c]
  * for `rows` rows: x fp16, rows x_stride elements apart (>= k, a multiple of
  * 8; x 16-byte aligned), y and residual fp16, rows y_stride / residual_stride
- * apart (>= n). bias and residual may be null; residual may be y itself.
- * Otherwise y overlaps no input. Products and sums in fp32 (the tensor
+ * apart (>= n). bias and residual may be null; residual may be y itself,
+ * with its stride. Otherwise y overlaps no input. Products and sums in fp32 (the tensor
  * cores' accumulation), one rounding, to fp16. Any k and n >= 1, rows from 0
  * (nothing is done) to 2^20; k, n and group_size as given to
  * tl_linear_pack. Rows do not affect one another, and a row's result

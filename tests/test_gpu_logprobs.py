@@ -233,3 +233,23 @@ def test_same_results_every_run_and_in_a_graph():
     again = call(logits, tokens, 20, "f16")
     assert all(torch.equal(a, b) for a, b in zip(first, again))
     assert torch.equal(lp, first[0]) and torch.equal(ent, first[1])
+
+
+@pytest.mark.parametrize("dtype,temperature", [("f16", 1e5), ("bf16", 3e37), ("f32", 3e37)])
+@pytest.mark.parametrize("vocab", [9, 5000])
+def test_masks_at_a_temperature_where_the_lowest_value_weighs(dtype, temperature, vocab):
+    """The type's lowest value then has a probability of its own; -inf never.
+
+    At 5000 tokens (10 elements a thread, 9 levels of joins, logarithms up to
+    12.3 in base 2) the roundings add up to 3.1e-6, below check()'s 4e-6."""
+    import torch
+    logits, tokens = make(5, vocab, dtype, 21)
+    low, nothing = torch.finfo(logits.dtype).min, float("-inf")
+    logits[0, ::2] = low
+    logits[1, ::2] = nothing
+    logits[2, ::3] = low
+    logits[2, 1::3] = nothing
+    logits[3] = low
+    logits[3, 0] = nothing
+    tokens[0], tokens[1], tokens[2], tokens[3] = 0, 0, 0, 1
+    check(logits, tokens, 5, dtype, temperature)

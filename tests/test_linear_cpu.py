@@ -70,6 +70,16 @@ def test_linear_refusals(gated):
         assert "strides" in status(lambda: call(residual=A, residual_stride=60))[1]
 
 
+def test_residual_in_place_keeps_the_stride():
+    """Row r of the residual would be another row's output otherwise."""
+    def call(rows, **kw):
+        T.linear(A, rows, A, 64, 64, 32, A, residual=A, **kw)
+
+    assert "in place" in status(lambda: call(4, residual_stride=72))[1]
+    assert "in place" in status(lambda: call(9, y_stride=128))[1]
+    call(0, residual_stride=72)  # nothing to do
+
+
 def test_logprob_refusals():
     def call(logits=A, rows=4, vocab=100, tokens=A, lp=A, **kw):
         T.token_logprobs(logits, rows, vocab, tokens, lp, **kw)

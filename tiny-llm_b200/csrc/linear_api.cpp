@@ -49,6 +49,8 @@ int linear(const char *ctx, tllm::LinearArgs a, cudaStream_t stream) {
         return set_thread_error(TL_ERR_INVALID_ARG, "%s: x_stride must be at least k and a multiple of 8", ctx);
     if (a.y_stride < a.n || (a.residual && a.residual_stride < a.n))
         return set_thread_error(TL_ERR_INVALID_ARG, "%s: the strides of output and residual must be at least n", ctx);
+    if (a.residual == a.y && a.residual_stride != a.y_stride)
+        return set_thread_error(TL_ERR_INVALID_ARG, "%s: a residual in place needs the output's stride", ctx);
     const int sms = tllm::current_device_sms();
     if (sms == 0) return set_thread_error(TL_ERR_NO_DEVICE, "%s: no CUDA device", ctx);
     const cudaError_t e = a.rows <= tllm::kLinearFewRows ? tllm::launch_linear(a, sms, stream)

@@ -155,8 +155,7 @@ __device__ __forceinline__ void add(Sums &s, float x, float c) {
 }
 
 // Two elements at a time, z by one packed FMA. nmc: -m c rounded once; what
-// that rounding shifts every z by is put right at the end (Sums are relative
-// to nmc / -c then, see unshift).
+// that rounding shifts every z by is put right at the end of each batch.
 struct Sums2 {
     uint64_t l, t;
 };
