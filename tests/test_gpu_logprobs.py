@@ -253,3 +253,22 @@ def test_masks_at_a_temperature_where_the_lowest_value_weighs(dtype, temperature
     logits[3, 0] = nothing
     tokens[0], tokens[1], tokens[2], tokens[3] = 0, 0, 0, 1
     check(logits, tokens, 5, dtype, temperature)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("vocab", [130, 300, 890, 1024])
+@pytest.mark.parametrize("top", [2, 20, 64])
+def test_many_candidates(dtype, vocab, top):
+    """Short rows and ties, whose list of candidates is long: few values, one
+    value, both zeros, masks that leave fewer than top."""
+    import torch
+    logits, tokens = make(7, vocab, dtype, 31)
+    logits[1] = (logits[1].float() / 2).round().to(logits.dtype)
+    logits[2] = 3.25
+    logits[3] = torch.where(torch.arange(vocab, device="cuda") % 3 == 1, 0.0, -0.0).to(logits.dtype)
+    logits[4, 1:] = float("-inf")
+    logits[5] = torch.finfo(logits.dtype).min
+    logits[5, vocab // 2:] = -1.0
+    logits[6, : vocab - 3] = float("-inf")
+    tokens[4], tokens[5] = 0, vocab - 1
+    check(logits, tokens, top, dtype)

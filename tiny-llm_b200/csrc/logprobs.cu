@@ -38,6 +38,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = kLogprobMaxTop;
 constexpr int kCand = 1024;
+constexpr int kRank = 160;             // candidates ranked without a cut; above kMaxTop
 constexpr int kMaxCluster = 8;
 constexpr int kMaxWarps = 16;
 constexpr int kMaxGroups = 128;        // of threads, for the bound; at least kMaxTop
@@ -185,6 +186,7 @@ struct Shared {
     Best cand[kCand];         // candidates; then the cluster's lists
     Best red[kMaxWarps];
     int rank[kMaxCluster * kMaxTop];
+    int tally[2][kMaxWarps];
 };
 static_assert(kMaxCluster * kMaxTop <= kCand, "the cluster's lists fit the candidates' place");
 
@@ -289,14 +291,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     }
     if (lane == 0) sh.sums[warp] = s;
     const int top = a.top;
-    // groups of 32, 16, 8, 4 or 2 lanes: half as many again as alternatives, so
-    // that the bound is not far below the n-th largest
+    // groups of 32 lanes or fewer: of those that hold elements half as many
+    // again as alternatives, so that the bound is not far below the n-th
+    // largest (with empty groups among the first n it would be -inf)
     int lanes = 32;
-    while (kThreads / lanes < top + top / 2) lanes >>= 1;
+    while (lanes > 1 && min(nvec, kThreads) / lanes < top + top / 2) lanes >>= 1;
+    const int groups = min(kThreads / lanes, kMaxGroups);
     if (top > 0) {
         float g = own;
         for (int o = 1; o < lanes; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if ((lane & (lanes - 1)) == 0) sh.gmax[tid / lanes] = g;
+        if ((lane & (lanes - 1)) == 0 && tid / lanes < groups) sh.gmax[tid / lanes] = g;
     }
     __syncthreads();
     if (warp == 0) {
@@ -310,7 +314,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
         if (lane == 0) sh.cta = t;
     }
     if (top > 0) {
-        const int groups = kThreads / lanes;
         const int at = tid - (kThreads - kMaxGroups);  // the last warps: warp 0 joins the sums
         if (at >= 0 && at < groups) {  // the group maximum of rank top - 1 (a NaN has rank 0: the row is answered with NaN)
             const float g = sh.gmax[at];
@@ -360,7 +363,50 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
             }
         }
         __syncthreads();
-        const int count = sh.count;
+        int count = sh.count;
+        if (count > kRank && count <= kCand) {
+            // A long list (ties, or a row too short for a close bound): ranking
+            // costs its square, so it is cut first, at a value found by halving
+            // the range of the order-preserving integers. top or more stay.
+            constexpr int kHold = kCand / kThreads;
+            Best h[kHold];
+            uint32_t key[kHold];
+#pragma unroll
+            for (int q = 0; q < kHold; ++q) {
+                const int j = tid + q * kThreads;
+                h[q] = j < count ? sh.cand[j] : Best{0.f, 0};
+                const uint32_t u = __float_as_uint(h[q].v + 0.f);  // -0 orders as +0
+                key[q] = j < count ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
+            }
+            uint32_t from = 1u, to = 0xffffffffu;  // the cut: `from` leaves `left` >= top, above `to` fewer than top
+            int left = count;
+            for (int step = 0; from < to && left > kRank; ++step) {
+                const uint32_t mid = from + (to - from) / 2 + 1;
+                int c1 = 0;
+#pragma unroll
+                for (int q = 0; q < kHold; ++q) c1 += key[q] >= mid;
+                c1 = __reduce_add_sync(0xffffffffu, c1);
+                if (lane == 0) sh.tally[step & 1][warp] = c1;
+                __syncthreads();
+                int all = 0;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) all += sh.tally[step & 1][w];
+                if (all >= top) {
+                    from = mid;
+                    left = all;
+                } else {
+                    to = mid - 1;
+                }
+            }
+            __syncthreads();  // every candidate is held, every tally read
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < kHold; ++q)
+                if (key[q] >= from) sh.cand[atomicAdd(&sh.count, 1)] = h[q];
+            __syncthreads();
+            count = sh.count;
+        }
         if (count <= kCand) {
             for (int j = tid; j < count; j += kThreads) {
                 const Best b = sh.cand[j];
