@@ -272,3 +272,17 @@ def test_many_candidates(dtype, vocab, top):
     logits[6, : vocab - 3] = float("-inf")
     tokens[4], tokens[5] = 0, vocab - 1
     check(logits, tokens, top, dtype)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,top", [(300, 150001, "f32", 20), (300, 150001, "f32", 2), (300, 300007, "f16", 9),
+                                                  (300, 30000, "f16", 5), (300, 30000, "f32", 64)])
+def test_long_slices_looked_at_again(rows, vocab, dtype, top):
+    """Slices of one batch of loads a thread to more than the kept maxima; the
+    largest sit together in one thread's elements of some rows."""
+    import torch
+    logits, tokens = make(rows, vocab, dtype, 41)
+    n = 16 // logits.element_size()
+    for r in range(0, rows, 7):  # the same thread's vectors, batch after batch
+        at = torch.arange(n * 3, vocab - 1, n * 256 * 8, device="cuda")[:top]
+        logits[r, at] = 30.0 - torch.arange(at.numel(), device="cuda").to(logits.dtype)
+    check(logits, tokens, top, dtype)
