@@ -286,3 +286,24 @@ def test_long_slices_looked_at_again(rows, vocab, dtype, top):
         at = torch.arange(n * 3, vocab - 1, n * 256 * 8, device="cuda")[:top]
         logits[r, at] = 30.0 - torch.arange(at.numel(), device="cuda").to(logits.dtype)
     check(logits, tokens, top, dtype)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 2e-5, 4e-5])
+@pytest.mark.parametrize("rows,vocab", [(1, 700), (1, 128256), (300, 1024), (300, 40003)])
+def test_fp16_large_logits_at_the_lowest_temperatures(rows, vocab, temperature):
+    """m log2(e) / T passes 2^31 (0 is clamped to 1e-5), where its fp32 rounding
+    is hundreds: maxima of both signs to the type's ends, ties at the maximum,
+    threads whose own maximum lies anywhere below it."""
+    import torch
+    maxima = [15104.0, 20000.0, 40000.0, 65504.0, -15104.0, -40000.0, -65472.0, 30000.0]
+    gen = torch.Generator(device="cuda").manual_seed(51)
+    for first in range(len(maxima) if rows == 1 else 1):
+        top = torch.tensor([maxima[(first + r) % len(maxima)] for r in range(rows)], device="cuda")[:, None]
+        body = -65504.0 + torch.rand(rows, vocab, device="cuda", generator=gen) * (top + 65504.0)
+        near = torch.randn(rows, vocab, device="cuda", generator=gen) * 3.0
+        narrow = (torch.arange(rows, device="cuda")[:, None] % 3 == 1) & (top > 0)
+        logits = torch.minimum(torch.where(narrow, near, body), top).half()
+        logits[:, 5:vocab:331] = top.half()  # ties
+        tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=gen).to(torch.int32)
+        tokens[::2] = 5
+        check(logits, tokens, 8, "f16", temperature)

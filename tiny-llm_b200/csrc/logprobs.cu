@@ -72,10 +72,16 @@ struct Vec<__half> {
         return max_nan(__low2float(m), __high2float(m));
     }
     static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-    // Whether, relative to a maximum m, an element at the type's lowest value
-    // weighs nothing: then -inf may be taken for it, which keeps every z finite
-    // without a comparison in fp32 for each.
-    static __device__ __forceinline__ bool lowest_is_nothing(float m, float c) { return (m + 65504.f) * c > 160.f; }
+    // Whether the packed pass holds, relative to a maximum m. An element at the
+    // type's lowest value has to weigh nothing: then -inf may be taken for it,
+    // which keeps every z finite without a comparison in fp32 for each. And
+    // m c, rounded once for all elements, may be off by one at most (half a
+    // unit of 2^24): the factor that puts the rounding right, 2^shift, stays
+    // within [1/2, 2]. At a temperature of 1e-5 m c reaches 9.4e9, its rounding
+    // 2^432, and no fp32 number holds that.
+    static __device__ __forceinline__ bool packed_pass(float m, float c) {
+        return (m + 65504.f) * c > 160.f && fabsf(m * c) < 16777216.f;
+    }
     static __device__ __forceinline__ uint4 raise(uint4 v) {
         const __half2 low = __halves2half2(__ushort_as_half(0xFBFF), __ushort_as_half(0xFBFF));
         __half2 *h = reinterpret_cast<__half2 *>(&v);
@@ -102,7 +108,7 @@ struct Vec<__nv_bfloat16> {
     }
     static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
     // (z of the lowest value is not finite for every c: clamped one by one)
-    static __device__ __forceinline__ bool lowest_is_nothing(float, float) { return false; }
+    static __device__ __forceinline__ bool packed_pass(float, float) { return false; }
     static __device__ __forceinline__ uint4 raise(uint4 v) { return v; }
 };
 template <>
@@ -120,7 +126,7 @@ struct Vec<float> {
     }
     static __device__ __forceinline__ float to_float(float v) { return v; }
     // (z of the lowest value is not finite for every c: clamped one by one)
-    static __device__ __forceinline__ bool lowest_is_nothing(float, float) { return false; }
+    static __device__ __forceinline__ bool packed_pass(float, float) { return false; }
     static __device__ __forceinline__ uint4 raise(uint4 v) { return v; }
 };
 
@@ -158,7 +164,8 @@ __device__ __forceinline__ void add(Sums &s, float x, float c) {
 }
 
 // Two elements at a time, z by one packed FMA. nmc: -m c rounded once; what
-// that rounding shifts every z by is put right at the end of each batch.
+// that rounding shifts every z by (packed_pass keeps it to one) is put right
+// at the end of each batch.
 struct Sums2 {
     uint64_t l, t;
 };
@@ -256,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
         // a batch of -inf alone moves the maximum to -FLT_MAX, not to -inf:
         // differences to it stay numbers
         rebase(s, max_nan(s.m, max_nan(m, -FLT_MAX)), c);
-        if (Vec<T>::lowest_is_nothing(s.m, c)) {
+        if (Vec<T>::packed_pass(s.m, c)) {
             const float nmc = -s.m * c, shift = fmaf(s.m, c, nmc);  // z of the maximum itself: the rounding of nmc
             const uint64_t c2 = ptx::f2_pack(c, c), nmc2 = ptx::f2_pack(nmc, nmc);
             Sums2 p = {0ull, 0ull}, q = {0ull, 0ull};
