@@ -307,3 +307,44 @@ def test_fp16_large_logits_at_the_lowest_temperatures(rows, vocab, temperature):
         tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=gen).to(torch.int32)
         tokens[::2] = 5
         check(logits, tokens, 8, "f16", temperature)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("temperature", [2.0, 4.0, 3e37, 1e38, 3e38])
+def test_differences_past_the_types_end(dtype, temperature):
+    """Logits whose difference overflows fp32 although, divided by T, it does
+    not: the small one then has a log probability, at T near 1e38 a weight too.
+    (Above 8e37 1 / T is subnormal: half a unit of it is 2.2e-7 of the value at
+    3e38, of |z| up to 3.3 in base 2 7e-7, inside check()'s 4e-6 + 4e-7 |z|.)"""
+    import torch
+    logits, _ = make(6, 700, dtype, 61)
+    big = torch.finfo(logits.dtype).max
+    logits[0] = -big
+    logits[0, 5] = big
+    logits[1, ::2], logits[1, 1::2] = big, -big
+    logits[2, ::3], logits[2, 1::3] = big * 0.75, -big * 0.625
+    logits[3, 9] = big
+    logits[4] = -big
+    logits[4, 600:] = big
+    logits[5, 3], logits[5, 4], logits[5, 5] = big, -big, float("-inf")
+    tokens = torch.tensor([0, 1, 1, 4, 10, 4], device="cuda", dtype=torch.int32)
+    check(logits, tokens, 4, dtype, temperature)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("vocab", [9, 5000])
+def test_infinite_temperature_is_uniform(dtype, vocab):
+    """softmax(logits / inf): the same for every finite logit, none for -inf."""
+    import torch
+    logits, _ = make(3, vocab, dtype, 62)
+    big = torch.finfo(logits.dtype).max
+    logits[0, 1], logits[0, 2] = big, -big
+    logits[1, ::2] = float("-inf")
+    logits[2] = float("-inf")
+    tokens = torch.tensor([2, 1, 0], device="cuda", dtype=torch.int32)
+    lp, ent, tt, tl = call(logits, tokens, 3, dtype, float("inf"))
+    allowed = torch.tensor([vocab, vocab // 2], dtype=torch.float64)
+    assert ((lp[:2].double().cpu() + allowed.log()).abs() <= 4e-6).all()
+    assert ((ent[:2].double().cpu() - allowed.log()).abs() <= 4e-5).all()
+    assert ((tl[:2].double().cpu() + allowed.log()[:, None]).abs() <= 4e-6).all()
+    assert lp[2] == float("-inf") and ent[2] == 0 and (tt[2] == -1).all()

@@ -28,6 +28,7 @@
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "kernels.h"
 #include "ptx.cuh"
@@ -137,27 +138,40 @@ struct Sums {
     float m, l, t;
 };
 
+// z of x. -inf (a masked logit, a thread that has seen nothing), and what is
+// far below, is held finite, so that 2^z = 0 and z 2^z = 0. kHalves, for c
+// below kFlat (T above 1.4e36): x - m may pass fp32's range where (x - m) c
+// does not, so it is taken by halves, which are exact and one FMA. From kFlat
+// on such a difference is 340 and more in z and its weight 0 either way. Two
+// instances of the kernel, since the FMA in place of the addition takes 8 %
+// more (2048 x 128256 bf16 103 us instead of 96), a branch per batch as much.
+constexpr float kFlat = 1e-36f;
+template <bool kHalves>
+__device__ __forceinline__ float z_of(float x, float m, float c) {
+    return fmaxf(kHalves ? fmaf(x, 0.5f, -0.5f * m) * (2.f * c) : (x - m) * c, -1e30f);
+}
+
 // Moves s to the maximum m >= s.m.
+template <bool kHalves>
 __device__ __forceinline__ void rebase(Sums &s, float m, float c) {
     if (m == s.m) return;
-    // s.m = -inf (nothing yet): d is held finite, l = t = 0 stay
-    const float d = fmaxf((s.m - m) * c, -1e30f), f = ptx::ex2(d);
+    const float d = z_of<kHalves>(s.m, m, c), f = ptx::ex2(d);  // (nothing yet: l = t = 0 stay)
     s.t = f * fmaf(d, s.l, s.t);
     s.l *= f;
     s.m = m;
 }
 
+template <bool kHalves>
 __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
     const float m = max_nan(a.m, b.m);
-    rebase(a, m, c);
-    rebase(b, m, c);
+    rebase<kHalves>(a, m, c);
+    rebase<kHalves>(b, m, c);
     return {m, a.l + b.l, a.t + b.t};
 }
 
+template <bool kHalves>
 __device__ __forceinline__ void add(Sums &s, float x, float c) {
-    // -inf (a masked logit, or one far below): 2^z = 0 and z held finite, so
-    // that z 2^z is 0 too
-    const float z = fmaxf((x - s.m) * c, -1e30f);
+    const float z = z_of<kHalves>(x, s.m, c);
     const float e = ptx::ex2(z);
     s.l += e;
     s.t = fmaf(e, z, s.t);
@@ -201,7 +215,7 @@ static_assert(kMaxCluster * kMaxTop <= kCand, "the cluster's lists fit the candi
 
 // kThreads: 512 where few CTAs share the device, 256 (four CTAs an SM) where
 // the end of one row has to hide behind the passes of others.
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool kHalves>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(const __grid_constant__ LogprobArgs a) {
     constexpr int N = Vec<T>::kN, kWarps = kThreads / 32;
     constexpr int kU = kThreads == 256 ? 8 : 4;  // vectors in flight per thread
@@ -241,8 +255,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     if (single >= 0) {
         const float v = Vec<T>::to_float(x[single]);
         own = v;
-        rebase(s, max_nan(fmaxf(v, -FLT_MAX), v), c);
-        add(s, v, c);
+        rebase<kHalves>(s, max_nan(fmaxf(v, -FLT_MAX), v), c);
+        add<kHalves>(s, v, c);
     }
     const bool once = nvec <= kThreads * kU;  // one round: the elements stay in registers
     uint4 v[kU];
@@ -262,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
         }
         // a batch of -inf alone moves the maximum to -FLT_MAX, not to -inf:
         // differences to it stay numbers
-        rebase(s, max_nan(s.m, max_nan(m, -FLT_MAX)), c);
+        rebase<kHalves>(s, max_nan(s.m, max_nan(m, -FLT_MAX)), c);
         if (Vec<T>::packed_pass(s.m, c)) {
             const float nmc = -s.m * c, shift = fmaf(s.m, c, nmc);  // z of the maximum itself: the rounding of nmc
             const uint64_t c2 = ptx::f2_pack(c, c), nmc2 = ptx::f2_pack(nmc, nmc);
@@ -292,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
                     float f[N];
                     Vec<T>::load(v[u], f);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) add(s, f[e], c);
+                    for (int e = 0; e < N; ++e) add<kHalves>(s, f[e], c);
                 }
         }
     }
@@ -302,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     for (int o = 16; o > 0; o >>= 1) {
         const Sums b = {__shfl_down_sync(0xffffffffu, s.m, o), __shfl_down_sync(0xffffffffu, s.l, o),
                         __shfl_down_sync(0xffffffffu, s.t, o)};
-        s = join(s, b, c);
+        s = join<kHalves>(s, b, c);
     }
     if (lane == 0) sh.sums[warp] = s;
     const int top = a.top;
@@ -324,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
         for (int o = kWarps / 2; o > 0; o >>= 1) {
             const Sums b = {__shfl_down_sync(0xffffffffu, t.m, o), __shfl_down_sync(0xffffffffu, t.l, o),
                             __shfl_down_sync(0xffffffffu, t.t, o)};
-            t = join(t, b, c);
+            t = join<kHalves>(t, b, c);
         }
         if (lane == 0) sh.cta = t;
     }
@@ -500,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
             for (int o = kMaxCluster / 2; o > 0; o >>= 1) {
                 const Sums b = {__shfl_down_sync(0xffffffffu, t.m, o), __shfl_down_sync(0xffffffffu, t.l, o),
                                 __shfl_down_sync(0xffffffffu, t.t, o)};
-                t = join(t, b, c);
+                t = join<kHalves>(t, b, c);
             }
             all = {__shfl_sync(0xffffffffu, t.m, 0), __shfl_sync(0xffffffffu, t.l, 0), __shfl_sync(0xffffffffu, t.t, 0)};
             if (top > 0) {
@@ -544,7 +558,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
         auto logprob = [&](float v) {
             if (bad) return nan;
             if (none || v == -INFINITY) return -INFINITY;
-            return (v - all.m) * a.inv_temperature - log2l * kLn2;  // the difference may reach the type's end: no log2 form
+            // the difference may pass the type's end: by halves, and no log2 form
+            return fmaf(v, 0.5f, -0.5f * all.m) * a.inv_temperature * 2.f - log2l * kLn2;
         };
         if (tid == 0) {
             if (a.logprobs) {
@@ -564,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprobs_kernel(con
     if (split > 1) cluster.sync();  // no CTA leaves while rank 0 may still read its shared memory
 }
 
-template <typename T, int kThreads>
+template <typename T, int kThreads, bool kHalves>
 cudaError_t launch_n(const LogprobArgs &a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.rows * (unsigned)a.split);
@@ -578,12 +593,14 @@ cudaError_t launch_n(const LogprobArgs &a, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, kThreads>, a);
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, kThreads, kHalves>, a);
 }
 
 template <typename T>
 cudaError_t launch_t(const LogprobArgs &a, int num_sms, cudaStream_t s) {
-    return (long long)a.rows * a.split > 2ll * num_sms ? launch_n<T, 256>(a, s) : launch_n<T, 512>(a, s);
+    if constexpr (!std::is_same_v<T, __half>)  // (fp16 differences stay inside fp32's range)
+        if (a.scale_log2 < kFlat) return launch_n<T, 512, true>(a, s);
+    return (long long)a.rows * a.split > 2ll * num_sms ? launch_n<T, 256, false>(a, s) : launch_n<T, 512, false>(a, s);
 }
 
 }  // namespace
