@@ -267,7 +267,8 @@ enum tl_dtype { TL_F16 = 0, TL_BF16 = 1, TL_F32 = 2 };
  * p = softmax(logits / T), T = temperature clamped to >= 1e-5 as the
  * sampler's: logprobs[r] = log p(tokens[r]), entropy[r] = -sum p log p (both
  * natural), top_tokens/top_logprobs [rows][top_n] the largest logits in
- * descending order, ties by ascending index, top_n 0..64. Sums in fp32. A
+ * descending order, ties by ascending index, top_n 0..64, vocab up to
+ * 2^31 - 1024. Sums in fp32. A
  * logit of -inf has probability 0: its log probability is -inf, it adds
  * nothing to the entropy and is no alternative; places without one hold
  * (-1, -inf). A row of nothing but -inf: log probability -inf, entropy 0. A

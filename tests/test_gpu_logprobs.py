@@ -348,3 +348,18 @@ def test_infinite_temperature_is_uniform(dtype, vocab):
     assert ((ent[:2].double().cpu() - allowed.log()).abs() <= 4e-5).all()
     assert ((tl[:2].double().cpu() + allowed.log()[:, None]).abs() <= 4e-6).all()
     assert lp[2] == float("-inf") and ent[2] == 0 and (tt[2] == -1).all()
+
+
+def test_the_longest_row():
+    """As many equal logits as a row may have: the list of candidates
+    overflows, and the search in its place steps past the last index. (The
+    sums are whole numbers; the logarithm's and the product's roundings are
+    2.3e-6 at 21.5.)"""
+    import torch
+    vocab = 2**31 - 1024
+    logits = torch.full((1, vocab), 1.0, device="cuda", dtype=torch.float16)
+    tokens = torch.tensor([vocab - 1], device="cuda", dtype=torch.int32)
+    lp, ent, tt, tl = call(logits, tokens, 2, "f16")
+    want = -np.log(vocab)
+    assert abs(lp.item() - want) <= 4e-6 and abs(ent.item() + want) <= 4e-5
+    assert tt.tolist() == [[0, 1]] and (tl.double() - want).abs().max() <= 4e-6

@@ -102,6 +102,13 @@ def test_logprob_refusals():
     assert "aligned" in status(lambda: call(tokens=A + 2))[1]
 
 
+def test_logprob_rows_whose_indices_would_wrap():
+    """The search through a slice steps by 512 elements: past 2^31 from here on."""
+    for vocab in (2**31 - 1023, 2**31 - 1):
+        kind, text = status(lambda: T.token_logprobs(A, 1, vocab, A, A))
+        assert kind is T.Unsupported and "vocab" in text
+
+
 def test_without_a_device():
     """Where there is no device the calls say so."""
     import torch

@@ -258,6 +258,7 @@ cudaError_t launch_linear_pack(const int8_t *w, const void *s, const int8_t *w2,
 
 // Log probabilities of one given token per row, entropy and alternatives.
 constexpr int kLogprobMaxTop = 64;
+constexpr int kLogprobMaxVocab = 0x7fffffff - 1023;  // an index may step past the row's end by a CTA's threads
 struct LogprobArgs {
     const void *logits;
     long long row_stride;     // elements

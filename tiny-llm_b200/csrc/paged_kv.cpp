@@ -1364,6 +1364,8 @@ int tl_token_logprobs(const void *logits, int dtype, long long row_stride, int r
     if (top_n < 0 || top_n > tllm::kLogprobMaxTop || rows > (1 << 27))
         return set_thread_error(TL_ERR_UNSUPPORTED, "tokenLogprobs: top_n must be 0..%d and rows at most 2^27",
                                 tllm::kLogprobMaxTop);
+    if (vocab > tllm::kLogprobMaxVocab)
+        return set_thread_error(TL_ERR_UNSUPPORTED, "tokenLogprobs: vocab must be at most 2^31 - 1024");
     if (rows == 0) return TL_OK;
     if (!logits) return set_thread_error(TL_ERR_INVALID_ARG, "tokenLogprobs: logits is null");
     if (logprobs && !tokens) return set_thread_error(TL_ERR_INVALID_ARG, "tokenLogprobs: tokens is null");
