@@ -118,9 +118,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                 ptx::tma_load_2d(dst, &xmap, bar, k0, 0, keep);
                 ptx::tma_load_2d(dst + kXHalf, &xmap, bar, k0 + 64, 0, keep);
             }
-            if (issued < count)  // gave up: the copies in flight land (or a bounded wait passes) before the CTA goes on
-                for (int i = max(0, issued - kNS); i < issued; ++i)
-                    ptx::mbar_wait_cycles(full_u + 8 * (i % kNS), (uint32_t)((i / kNS) & 1), kWait);
+            // whoever gave up, the last copies land (or a bounded wait passes) before the CTA goes on
+            for (int i = max(0, issued - kNS); i < issued; ++i)
+                ptx::mbar_wait_cycles(full_u + 8 * (i % kNS), (uint32_t)((i / kNS) & 1), kWait);
         }
         __syncwarp();
     } else {

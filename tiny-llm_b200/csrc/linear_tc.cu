@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     const uint32_t dempty_u = dfull_u + 16;                // [2] ... and drained
     const uint32_t done_u = dempty_u + 16;                 // every UMMA complete
     __shared__ uint32_t s_tmem;
+    __shared__ int s_failed;  // a drain's wait gave up (csplit > 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int RT = a.row_tile;  // rows of a tile, a multiple of 32
@@ -272,6 +273,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
         }
         ptx::mbar_init(done_u, C::kIssue);
         ptx::fence_barrier_init();
+        s_failed = 0;
     }
     if (warp == C::kMma) ptx::tmem_alloc(ptx::smem_u32(&s_tmem), C::kTmemCols);
     ptx::tc_fence_before_sync();
@@ -335,9 +337,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                     w1 += unit;
                 }
             }
-            if (!ok)  // the copies in flight land (or a bounded wait passes) before the CTA goes on
-                for (int i = max(0, issued - NS); i < issued; ++i)
-                    ptx::mbar_wait_cycles(full_u + 8 * (i % NS), (uint32_t)((i / NS) & 1), kWait);
+            // whoever gave up, the last copies land (or a bounded wait passes) before the CTA goes on
+            for (int i = max(0, issued - NS); i < issued; ++i)
+                ptx::mbar_wait_cycles(full_u + 8 * (i % NS), (uint32_t)((i / NS) & 1), kWait);
         }
     } else if (warp >= C::kMma) {
         if (lane == 0) {
@@ -486,12 +488,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(dempty_u + 8 * dd.s);
             }
-            if (!ok) {
-                const float nan = __int_as_float(0x7fffffff);
-#pragma unroll
-                for (int i = 0; i < C::kAcc; ++i) acc[i] = nan;
-            }
             if (csplit > 1) {  // the CTA's one tile: its sums to the ring (every step is consumed)
+                if (!ok) s_failed = 1;
                 float *part = reinterpret_cast<float *>(smem);
 #pragma unroll
                 for (int i = 0; i < C::kAcc; ++i)
@@ -524,6 +522,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
                 uint32_t v[16];
                 tmem_ld16(tsum + (uint32_t)(c * 16), v);
                 tmem_wait_ld16(v);
+                if (!ok)  // not from TMEM, where a UMMA may still be adding
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = 0x7fffffffu;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) st[i * kOutPitch + lane] = __uint_as_float(v[i]);
                 __syncwarp();
@@ -552,6 +553,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kPerSm)
     if (csplit > 1) {
         // ---- the parts of K, in rank order, and the epilogue ----
         cg::cluster_group cluster = cg::this_cluster();
+        if (s_failed)  // NaN, not a wrong number; here, where no copy lands in the ring any more
+            for (int i = threadIdx.x; i < RT * kM; i += C::kThreads)
+                reinterpret_cast<float *>(smem)[i] = __int_as_float(0x7fffffff);
         __syncwarp();
         cluster.sync();
         const TilePos p = tile_pos(first, ntiles, nrt);
