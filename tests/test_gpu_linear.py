@@ -445,3 +445,85 @@ def test_logits_written_between_two_readers(rows):
     torch.cuda.synchronize()
     for g, r in zip(got, ref):
         assert all(torch.equal(g[i], r[i % 3]) for i in range(n))
+
+
+def exact_weight(k, n, group, gen):
+    """A weight whose scales are powers of two, 2^-6 to 2^-3."""
+    import torch
+    W = Weight(k, n, group, gen)
+    W.s = torch.exp2(torch.randint(-6, -2, W.s.shape, device="cuda", generator=gen).float()).half()
+    W.v = W.w.double() * W.s.double().repeat_interleave(group, 0)[:k]
+    return W
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 40, 64, 130])
+@pytest.mark.parametrize("k,n,group", [(8192, 200, 128), (8191, 65, 32), (5001, 129, 64), (300, 1000, 32)])
+def test_exact_sums(rows, k, n, group):
+    """Small whole activations and scales that are powers of two: every sum,
+    in any order, is a whole number of 2^-6 below 2^24 of them, so fp32 holds
+    it exactly and the output is the exact sum rounded once, bit for bit. A
+    lost or doubled row of K, or another group's scale, shows."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(k + rows)
+    W = exact_weight(k, n, group, gen)
+    packed = pack(k, n, group, W)
+    x = make_x(rows, k, gen)
+    x[:, :k] = torch.randint(-3, 4, (rows, k), device="cuda", generator=gen).half()
+    x[:, k - 1] = 3.0  # the last row of K weighs in every output
+    xd = x[:, :k].double()
+    assert (xd.abs() @ W.v.abs()).max() * 64 < 2**24
+    y = torch.empty(rows, n, device="cuda", dtype=torch.float16)
+    T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr(), x_stride=x.stride(0))
+    torch.cuda.synchronize()
+    assert torch.equal(y, (xd @ W.v).half())
+
+
+@pytest.mark.parametrize("rows", [1, 8, 40, 130])
+@pytest.mark.parametrize("k,n,group", [(4096, 100, 128), (4095, 33, 32)])
+def test_exact_gated_sums(rows, k, n, group):
+    """The same of a gated pair: both sums are exact (17 bits), their product
+    is rounded to fp32 and then to fp16, as here."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(k + rows + 1)
+    A, B = exact_weight(k, n, group, gen), exact_weight(k, n, group, gen)
+    packed = pack(k, n, group, A, B)
+    x = make_x(rows, k, gen)
+    x[:, :k] = torch.randint(-1, 2, (rows, k), device="cuda", generator=gen).half() / 16
+    x[:, k - 1] = 0.0625
+    xd = x[:, :k].double()
+    assert max((xd.abs() @ M.v.abs()).max() for M in (A, B)) * 1024 < 2**24
+    y = torch.empty(rows, n, device="cuda", dtype=torch.float16)
+    T.linear_gated(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr(), activation=T.TL_ACT_RELU,
+                   x_stride=x.stride(0))
+    torch.cuda.synchronize()
+    ref = torch.relu(xd @ A.v) * (xd @ B.v)
+    assert torch.equal(y, ref.float().half())
+
+
+@pytest.mark.parametrize("rows", [1, 8, 33, 64, 200])
+@pytest.mark.parametrize("k,group", [(512, 32), (4096, 128), (8192, 64)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_no_weight_is_rounded(rows, k, group, gated):
+    """The outputs' rms error is the final rounding's alone. Next to that
+    rounding (2.1e-4 of the value, rms) the fp32 sums add sqrt(k) 2^-23 at
+    most (1.1e-5 at 8192: 0.2 %, in rms); weights rounded to fp16 first would
+    add as much again (41 % in rms). The limit is 5 %."""
+    import torch
+    n = 20000 // rows + 7
+    gen = torch.Generator(device="cuda").manual_seed(k + rows)
+    A = Weight(k, n, group, gen)
+    B = Weight(k, n, group, gen) if gated else None
+    packed = pack(k, n, group, A, B)
+    x = make_x(rows, k, gen)
+    y = torch.empty(rows, n, device="cuda", dtype=torch.float16)
+    xd = x[:, :k].double()
+    ref = xd @ A.v
+    if gated:
+        T.linear_gated(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr(), activation=T.TL_ACT_NONE,
+                       x_stride=x.stride(0))
+        ref = ref * (xd @ B.v)
+    else:
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr(), x_stride=x.stride(0))
+    torch.cuda.synchronize()
+    rms = (y.double() - ref).square().mean().sqrt()
+    assert rms <= 1.05 * (ref.half().double() - ref).square().mean().sqrt()
