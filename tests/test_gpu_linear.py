@@ -527,3 +527,112 @@ def test_no_weight_is_rounded(rows, k, group, gated):
     torch.cuda.synchronize()
     rms = (y.double() - ref).square().mean().sqrt()
     assert rms <= 1.05 * (ref.half().double() - ref).square().mean().sqrt()
+
+
+@pytest.mark.parametrize("rows,k,n,group", [(3, 1 << 20, 65, 128), (33, 1 << 20, 40, 32), (2, 40, 1 << 22, 32),
+                                            (40, 33, 1 << 22, 64), (1 << 20, 24, 9, 32)])
+def test_the_largest_dimensions(rows, k, n, group):
+    """k, n and rows at their documented limits, on sums that are exact."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    W = Weight.__new__(Weight)
+    W.w = torch.randint(-128, 128, (k, n), device="cuda", generator=gen, dtype=torch.int8)
+    W.s = torch.full((-(-k // group), n), 0.125, device="cuda", dtype=torch.float16)
+    W.s[:, ::2] = 0.25
+    packed = pack(k, n, group, W)
+    x = make_x(rows, k, gen)
+    x[:, :k] = torch.randint(0, 50, (rows, k), device="cuda", generator=gen) == 0  # zeros and ones: |sum| < 2^21
+    x[:, 0] = x[:, k - 1] = 1.0
+    y = torch.full((rows + 1, n), 7.0, device="cuda", dtype=torch.float16)
+    T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y.data_ptr(), x_stride=x.stride(0))
+    torch.cuda.synchronize()
+    scale = W.s[0].double()
+    for j in range(0, n, 1 << 19):  # (the scales of a column are alike; its product is a whole number)
+        part = x[:, :k].double() @ W.w[:, j:j + (1 << 19)].double() * scale[j:j + (1 << 19)]
+        assert torch.equal(y[:rows, j:j + (1 << 19)], part.half())
+    assert (y[rows] == 7.0).all()
+
+
+@pytest.mark.parametrize("rows", [2, 33, 150])
+def test_a_capture_that_forks_and_joins(rows):
+    """A product captured behind two streams' kernels, one its input, one its
+    residual, and read by kernels of both."""
+    import torch
+    k, n, group = 1024, 256, 64
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    W = Weight(k, n, group, gen)
+    packed = pack(k, n, group, W)
+    x, x2 = make_x(rows, k, gen), make_x(rows, n, gen)
+    P = Weight(n, n, group, gen)
+    packed2 = pack(n, n, group, P)
+    side = torch.cuda.Stream()
+
+    def chain(out):
+        main = torch.cuda.current_stream()
+        res, y = out
+        side.wait_stream(main)
+        T.linear(x2.data_ptr(), rows, packed2.data_ptr(), n, n, group, res.data_ptr(), stream=side.cuda_stream)
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y[0].data_ptr(), stream=main.cuda_stream)
+        main.wait_stream(side)
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y[1].data_ptr(), residual=res.data_ptr(),
+                 stream=main.cuda_stream)
+        side.wait_stream(main)
+        T.linear(y[1].data_ptr(), rows, packed2.data_ptr(), n, n, group, y[2].data_ptr(), stream=side.cuda_stream)
+        T.linear(y[1].data_ptr(), rows, packed2.data_ptr(), n, n, group, y[3].data_ptr(), residual=y[0].data_ptr(),
+                 stream=main.cuda_stream)
+        main.wait_stream(side)
+
+    def fresh():
+        return (torch.zeros(rows, n, device="cuda", dtype=torch.float16),
+                torch.zeros(4, rows, n, device="cuda", dtype=torch.float16))
+
+    ref, got = fresh(), fresh()
+    chain(ref)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain(got)
+    for _ in range(20):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    assert (ref[1].abs().amax((1, 2)) > 0).all()
+
+
+def test_beside_prefill_attention():
+    """Products of every row tile on two streams while a third runs the
+    prefill kernel, which takes all of an SM's TMEM: each gives what it gives
+    alone."""
+    import torch
+    from gpu_helpers import Run
+    r = Run.create(1, 8, 2, 128, 16, 1024, 2)
+    sid = r.allocate(1024)
+    r.prefill(sid, 900, 5)
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    q = torch.randn(900, 8, 128, device="cuda", generator=gen).half()
+    o = torch.empty(12, 900, 8, 128, device="cuda", dtype=torch.float16)
+    k, n, group = 2048, 1500, 128
+    W = Weight(k, n, group, gen)
+    packed = pack(k, n, group, W)
+    jobs = []
+    for rows in (4, 20, 32, 50, 64, 100, 300):
+        x = make_x(rows, k, gen)
+        ref = torch.empty(rows, n, device="cuda", dtype=torch.float16)
+        T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, ref.data_ptr())
+        jobs.append((rows, x, ref, torch.empty(12, rows, n, device="cuda", dtype=torch.float16)))
+    alone = torch.empty_like(o[0])
+    r.cache.prefill_attention(0, q.data_ptr(), alone.data_ptr(), [sid], [900])
+    torch.cuda.synchronize()
+    a, b, c = (torch.cuda.Stream() for _ in range(3))
+    for i in range(12):
+        r.cache.prefill_attention(0, q.data_ptr(), o[i].data_ptr(), [sid], [900], stream=a.cuda_stream)
+        for j, (rows, x, _, y) in enumerate(jobs):
+            T.linear(x.data_ptr(), rows, packed.data_ptr(), k, n, group, y[i].data_ptr(),
+                     stream=(b if (i + j) % 2 else c).cuda_stream)
+    torch.cuda.synchronize()
+    r.cache.sync_check()
+    assert all(torch.equal(o[i], alone) for i in range(12))
+    for _, _, ref, y in jobs:
+        assert all(torch.equal(y[i], ref) for i in range(12))

@@ -363,3 +363,18 @@ def test_the_longest_row():
     want = -np.log(vocab)
     assert abs(lp.item() - want) <= 4e-6 and abs(ent.item() + want) <= 4e-5
     assert tt.tolist() == [[0, 1]] and (tl.double() - want).abs().max() <= 4e-6
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_many_short_rows(dtype):
+    """2^20 rows of a few logits."""
+    import torch
+    rows, vocab = 1 << 20, 5
+    logits, tokens = make(rows, vocab, dtype, 71, pad=2)
+    lp, ent, tt, tl = call(logits, tokens, 2, dtype)
+    lsm = torch.log_softmax(logits.double(), 1)
+    assert ((lp.double() - lsm.gather(1, tokens.long()[:, None])[:, 0]).abs() <= 1e-5).all()
+    assert ((ent.double() + (lsm.exp() * lsm).sum(1)).abs() <= 4e-5).all()
+    order = torch.sort(logits.float(), dim=1, descending=True, stable=True).indices[:, :2]
+    assert torch.equal(tt.long(), order)
+    assert ((tl.double() - lsm.gather(1, order)).abs() <= 1e-5).all()
