@@ -268,15 +268,15 @@ enum tl_dtype { TL_F16 = 0, TL_BF16 = 1, TL_F32 = 2 };
  * sampler's: logprobs[r] = log p(tokens[r]), entropy[r] = -sum p log p (both
  * natural), top_tokens/top_logprobs [rows][top_n] the largest logits in
  * descending order, ties by ascending index, top_n 0..64, vocab up to
- * 2^31 - 1024. Sums in fp32. A
- * logit of -inf has probability 0: its log probability is -inf, it adds
- * nothing to the entropy and is no alternative; places without one hold
- * (-1, -inf). A row of nothing but -inf: log probability -inf, entropy 0. A
+ * 2^31 - 1024. Sums in fp32. A logit of -inf has probability 0: its log
+ * probability is -inf, it adds nothing to the entropy and is no alternative;
+ * places without one hold (-1, -inf). A row of nothing but -inf: log probability -inf, entropy 0. A
  * row that holds a NaN or +inf: NaN, and alternatives (-1, NaN). A negative
  * token (padding) gives 0, one >= vocab NaN. All pointers are device memory,
- * tokens int32; logprobs, entropy and either top output may be null,
- * though not all of them; tokens is read for logprobs alone. No handle: the call runs on the
- * current device, errors are read with tl_last_error(NULL). */
+ * tokens int32; logprobs, entropy and either top output may be null, though
+ * not all of them; tokens is read for logprobs alone. No output overlaps an
+ * input or another output. No handle: the call runs on the current device,
+ * errors are read with tl_last_error(NULL). */
 int tl_token_logprobs(const void *logits, int dtype, long long row_stride, int rows, int vocab, float temperature,
                       const int *tokens, float *logprobs, float *entropy, int top_n, int *top_tokens,
                       float *top_logprobs, tl_stream_t stream);
@@ -314,11 +314,15 @@ int tl_linear_pack(const int8_t *w, const void *scales, const int8_t *w_up, cons
  * for `rows` rows: x fp16, rows x_stride elements apart (>= k, a multiple of
  * 8; x 16-byte aligned), y and residual fp16, rows y_stride / residual_stride
  * apart (>= n). bias and residual may be null; residual may be y itself,
- * with its stride. Otherwise y overlaps no input. Products and sums in fp32 (the tensor
- * cores' accumulation), one rounding, to fp16. Any k and n >= 1, rows from 0
- * (nothing is done) to 2^20; k, n and group_size as given to
- * tl_linear_pack. Rows do not affect one another, and a row's result
- * depends on neither timing nor stream. */
+ * with its stride. Otherwise y overlaps no input. Products and sums in fp32
+ * (the tensor cores' accumulation), one rounding, to fp16. Any k and n >= 1,
+ * rows from 0 (nothing is done) to 2^20; k, n and group_size as given to
+ * tl_linear_pack. Rows do not affect one another's values, and a row's result
+ * depends on neither timing nor stream; their number chooses the order of the
+ * fp32 sums, so a row's last bit may differ between calls of other `rows`.
+ * The kernels' waits for their own copies and products are bounded, about 2 s
+ * each. One that gives up (a device that is stopped or failing) leaves NaN in
+ * the outputs it concerns; no status reports it, since the call has returned. */
 int tl_linear(const void *x, long long x_stride, int rows, const void *packed, int k, int n, int group_size,
               const void *bias, int activation, const void *residual, long long residual_stride, void *y,
               long long y_stride, tl_stream_t stream);

@@ -465,7 +465,9 @@ def pack_linear_weight(w_ptr, scales_ptr, k, n, group_size, out_ptr, w_up_ptr=0,
 def linear(x_ptr, rows, packed_ptr, k, n, group_size, y_ptr, bias=0, activation=TL_ACT_NONE, residual=0,
            x_stride=None, y_stride=None, residual_stride=None, stream=0):
     """tl_linear: act(x W + bias) + residual for `rows` fp16 rows over packed
-    W8A16 weights (strides in elements, None: rows of k or n)."""
+    W8A16 weights (strides in elements, None: rows of k or n). x_stride is a
+    multiple of 8: where k is not, two rows or more have to lie in padded
+    rows and x_stride has to be given."""
     lib = load()
     _check_thread(lib, lib.tl_linear(x_ptr, k if x_stride is None else x_stride, rows, packed_ptr, k, n, group_size,
                                      bias, activation, residual, n if residual_stride is None else residual_stride,
@@ -475,7 +477,7 @@ def linear(x_ptr, rows, packed_ptr, k, n, group_size, y_ptr, bias=0, activation=
 def linear_gated(x_ptr, rows, packed_ptr, k, n, group_size, y_ptr, activation=TL_ACT_SILU, bias=0, bias_up=0,
                  x_stride=None, y_stride=None, stream=0):
     """tl_linear_gated: act(x W + bias) * (x W_up + bias_up) over a pair of
-    weights packed together."""
+    weights packed together (x_stride as linear's)."""
     lib = load()
     _check_thread(lib, lib.tl_linear_gated(x_ptr, k if x_stride is None else x_stride, rows, packed_ptr, k, n,
                                            group_size, bias, bias_up, activation, y_ptr,
