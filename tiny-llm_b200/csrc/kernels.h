@@ -254,7 +254,7 @@ cudaError_t launch_linear(LinearArgs a, int num_sms, cudaStream_t s);     // up 
 cudaError_t launch_linear_tc(LinearArgs a, int num_sms, cudaStream_t s);  // more: linear_tc.cu
 // w2/s2: the other projection of a gated pair, or nullptr.
 cudaError_t launch_linear_pack(const int8_t *w, const void *s, const int8_t *w2, const void *s2, int k, int n, int group,
-                               void *out, cudaStream_t st);
+                               void *out, int num_sms, cudaStream_t st);
 
 // Log probabilities of one given token per row, entropy and alternatives.
 constexpr int kLogprobMaxTop = 64;

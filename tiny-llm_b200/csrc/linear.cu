@@ -328,9 +328,10 @@ cudaError_t launch_linear(LinearArgs a, int num_sms, cudaStream_t s) {
 }
 
 cudaError_t launch_linear_pack(const int8_t *w, const void *s, const int8_t *w2, const void *s2, int k, int n, int group,
-                               void *out, cudaStream_t st) {
-    linear_pack_kernel<<<148 * 8, 256, 0, st>>>(w, static_cast<const __half *>(s), w2, static_cast<const __half *>(s2), k,
-                                               n, group, static_cast<uint8_t *>(out));
+                               void *out, int num_sms, cudaStream_t st) {
+    linear_pack_kernel<<<num_sms * 8, 256, 0, st>>>(w, static_cast<const __half *>(s), w2,
+                                                   static_cast<const __half *>(s2), k, n, group,
+                                                   static_cast<uint8_t *>(out));
     return cudaGetLastError();
 }
 

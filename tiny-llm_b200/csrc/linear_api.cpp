@@ -89,8 +89,10 @@ int tl_linear_pack(const int8_t *w, const void *scales, const int8_t *w_up, cons
     };
     if (hits(w, wb) || hits(w_up, wb) || hits(scales, sb) || hits(scales_up, sb))
         return set_thread_error(TL_ERR_INVALID_ARG, "%s: source and destination overlap", ctx);
-    if (tllm::current_device_sms() == 0) return set_thread_error(TL_ERR_NO_DEVICE, "%s: no CUDA device", ctx);
-    const cudaError_t e = tllm::launch_linear_pack(w, scales, w_up, scales_up, k, n, group_size, packed, (cudaStream_t)stream);
+    const int sms = tllm::current_device_sms();
+    if (sms == 0) return set_thread_error(TL_ERR_NO_DEVICE, "%s: no CUDA device", ctx);
+    const cudaError_t e =
+        tllm::launch_linear_pack(w, scales, w_up, scales_up, k, n, group_size, packed, sms, (cudaStream_t)stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
         return set_thread_error(TL_ERR_CUDA, "%s: launch failed: %s", ctx, cudaGetErrorString(e));
