@@ -378,3 +378,20 @@ def test_many_short_rows(dtype):
     order = torch.sort(logits.float(), dim=1, descending=True, stable=True).indices[:, :2]
     assert torch.equal(tt.long(), order)
     assert ((tl.double() - lsm.gather(1, order)).abs() <= 1e-5).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("temperature", [2e36, 1e38])
+@pytest.mark.parametrize("rows,vocab", [(2, 128256), (300, 20011)])
+def test_long_rows_of_the_types_ends(dtype, temperature, rows, vocab):
+    """Differences past fp32's range over many batches, split rows and joins."""
+    import torch
+    logits, tokens = make(rows, vocab, dtype, 63)
+    big = torch.finfo(logits.dtype).max
+    gen = torch.Generator(device="cuda").manual_seed(64)
+    u = torch.rand(rows, vocab, device="cuda", generator=gen) * 2 - 1
+    logits[:] = (u * big).to(logits.dtype)
+    logits[:, 7::5] = float("-inf")
+    logits[:, 11], logits[:, vocab - 3] = big, -big
+    tokens[::2] = vocab - 3
+    check(logits, tokens, 8, dtype, temperature)
