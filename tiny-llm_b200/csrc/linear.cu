@@ -21,7 +21,9 @@
 //
 // The warps' sums meet in shared memory and, when K is split, the CTAs' in
 // distributed shared memory, both in a fixed order: the result does not
-// depend on timing. Waits are bounded; a CTA whose wait gives up writes NaN.
+// depend on timing. The mbarrier waits are bounded; a CTA whose wait gives up
+// writes NaN. The barriers of the CTA and the cluster have no limit of their
+// own: they wait for roles whose mbarrier waits all end.
 #include <algorithm>
 #include <atomic>
 #include <cooperative_groups.h>

@@ -34,8 +34,13 @@
 //
 // Too few tiles for the SMs: a cluster's CTAs share a tile's K and add their
 // sums in distributed shared memory, in rank order. No atomics, no workspace:
-// results do not depend on timing. Waits are bounded; a CTA whose wait gives
-// up writes NaN.
+// results do not depend on timing. The mbarrier waits are bounded; a CTA whose
+// wait gives up writes NaN. What has no limit of its own ends because what it
+// waits for does: the barriers of the CTA and the cluster wait for roles whose
+// mbarrier waits all end, and tcgen05.alloc for CTAs of the SM that hold
+// columns and wait for nobody who still needs some. (A kernel that waits for
+// this one was let in after every CTA here had its columns, and columns are
+// given back before the cluster's barriers.)
 #include <algorithm>
 #include <atomic>
 #include <cooperative_groups.h>
@@ -637,7 +642,9 @@ cudaError_t launch_t(const LinearArgs &a, unsigned grid, cudaStream_t s) {
 
 // Few rows: the weight stream asks for two CTAs' converters and issuers per SM
 // (10 warps of 96 registers each; 32 rows x 4096 x 14336 gated 27 us against
-// 31.6 with two issuers a CTA, whose 80 registers spill, and 36 with one CTA).
+// 31.6 with two issuers a CTA, whose 80 registers spill, and 36 with one CTA,
+// measured beside one another; the present build takes 28.7 to 33 by box and
+// clocks).
 // Many: the sums ask for drains (64 rows a thread; 80 and 96 measured 5 % and
 // more slower at 8192 x 4096 x 4096 and ragged sizes).
 using Small = Cfg<32, 2, 4, 4, 1, 2>;

@@ -5,20 +5,26 @@
 //   top        = the largest x_j, equal ones by their index
 // One pass over a row: every thread keeps the maximum of its elements and,
 // relative to it, the two sums (fp32, base 2), rescaled when the maximum
-// grows, so the row is read from HBM once and nothing of it is kept; the
-// logits' bytes bound it, closely followed by the instructions an element
-// takes (a conversion, the exponential, and half each of four packed ones).
-// Rows too few to fill the machine are split over the CTAs of a cluster,
-// which join in distributed shared memory.
+// grows, so the row is read from HBM once and nothing of it is kept. Many
+// rows run near the stream: 2048 x 128256 without alternatives 92 us in fp16
+// (packed arithmetic), 96 in bf16 (0.87 and 0.84 of the measured copy rate),
+// 1024 rows of fp32 80 us (1.0). Rows too few to fill the machine are split
+// over the CTAs of a cluster, which join in distributed shared memory.
 //
-// The alternatives cost next to nothing in the pass: of the maxima of 16 to
-// 128 groups of threads the n-th largest is a lower bound of the n-th largest
-// logit, and only threads whose own maximum reaches it can hold one of the n.
-// Their elements are looked at again (in registers where they fit, else those
+// The alternatives add little to the pass: of the maxima of 8 to 128 groups
+// of threads the n-th largest is a lower bound of the n-th largest logit, and
+// only threads whose own maximum reaches it can hold one of the n. What comes
+// after the pass is serial, and with few or short rows most of the call: their
+// elements are looked at again (in registers where they fit, else those
 // batches whose maximum, kept in shared memory, reaches the bound, from L2),
 // the ones that reach the bound are listed and ranked by counting, a long list
-// after a cut. A list that overflows (thousands of equal logits) is replaced by n searches of the
-// slice for the largest element behind the last one found.
+// after a cut. One row of 128256 fp16 logits takes 4.9 us without
+// alternatives, 8.0 with 5, 10.2 with 20, 16.8 with 64.
+// A list that overflows is replaced by n searches of the slice for the largest
+// element behind the last one found. Thousands of equal logits bring that
+// about, a finite mask value that leaves fewer tokens than alternatives among
+// them: 300 rows of 128256 with five tokens over the type's lowest value, 20
+// alternatives, take 1.18 ms; with -inf in the mask's place 0.05.
 //
 // Sums are combined in a fixed order: a row's result does not depend on
 // timing.
