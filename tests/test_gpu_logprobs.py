@@ -395,3 +395,19 @@ def test_long_rows_of_the_types_ends(dtype, temperature, rows, vocab):
     logits[:, 11], logits[:, vocab - 3] = big, -big
     tokens[::2] = vocab - 3
     check(logits, tokens, 8, dtype, temperature)
+
+
+@pytest.mark.parametrize("dtype,temperature", [("bf16", 1.0), ("f32", 1.0), ("f16", 1e4)])
+@pytest.mark.parametrize("rows,vocab", [(300, 128256), (450, 160001)])
+def test_rows_of_alike_weights(dtype, temperature, rows, vocab):
+    """The largest logit in every thread's first vector and one value for all
+    the others, 500 to 625 to a thread, so that every addition to a running sum
+    could round the same way: 7.7e-6 of it, one by one. By batches of at most 64 it is 1e-6, and with 16
+    batches, 11 joins (2^-24 each, 1.6e-6) and the logarithm's roundings (at 12:
+    1.2e-6) 3.8e-6, below check()'s 4e-6 + 4e-7 |z|."""
+    import torch
+    logits, tokens = make(rows, vocab, dtype, 81)
+    level = -(torch.arange(rows, device="cuda") % 50 + 14).float() / 64  # weights 0.37 to 0.8
+    logits[:] = (level * temperature)[:, None].to(logits.dtype)
+    logits[:, :2048] = 0.0
+    check(logits, tokens, 0, dtype, temperature)
