@@ -270,13 +270,14 @@ enum tl_dtype { TL_F16 = 0, TL_BF16 = 1, TL_F32 = 2 };
  * descending order, ties by ascending index, top_n 0..64, vocab up to
  * 2^31 - 1024. Sums in fp32. A logit of -inf has probability 0: its log
  * probability is -inf, it adds nothing to the entropy and is no alternative;
- * places without one hold (-1, -inf). A row of nothing but -inf: log probability -inf, entropy 0. A
- * row that holds a NaN or +inf: NaN, and alternatives (-1, NaN). A negative
- * token (padding) gives 0, one >= vocab NaN. All pointers are device memory,
- * tokens int32; logprobs, entropy and either top output may be null, though
- * not all of them; tokens is read for logprobs alone. No output overlaps an
- * input or another output. No handle: the call runs on the current device,
- * errors are read with tl_last_error(NULL). */
+ * places without one hold (-1, -inf). A row of nothing but -inf: log
+ * probability -inf, entropy 0. A row that holds a NaN or +inf: NaN, and
+ * alternatives (-1, NaN). A negative token (padding) gives 0, one >= vocab
+ * NaN. All pointers are device memory, tokens int32; logprobs, entropy and
+ * either top output may be null, though not all of them; tokens is read for
+ * logprobs alone. No output overlaps an input or another output. No handle:
+ * the call runs on the current device, errors are read with
+ * tl_last_error(NULL). */
 int tl_token_logprobs(const void *logits, int dtype, long long row_stride, int rows, int vocab, float temperature,
                       const int *tokens, float *logprobs, float *entropy, int top_n, int *top_tokens,
                       float *top_logprobs, tl_stream_t stream);

@@ -82,10 +82,10 @@ struct Vec<__half> {
     // Whether the packed pass holds, relative to a maximum m. An element at the
     // type's lowest value has to weigh nothing: then -inf may be taken for it,
     // which keeps every z finite without a comparison in fp32 for each. And
-    // m c, rounded once for all elements, may be off by one at most (half a
-    // unit of 2^24): the factor that puts the rounding right, 2^shift, stays
-    // within [1/2, 2]. At a temperature of 1e-5 m c reaches 9.4e9, its rounding
-    // 2^432, and no fp32 number holds that.
+    // m c, rounded once for all elements, may be off by a half at most (below
+    // 2^24 fp32's unit is one or less): the factor that puts the rounding
+    // right, 2^shift, stays within [0.7, 1.42]. At a temperature of 1e-5 m c
+    // reaches 9.4e9 and shift 432, whose power no fp32 number holds.
     static __device__ __forceinline__ bool packed_pass(float m, float c) {
         return (m + 65504.f) * c > 160.f && fabsf(m * c) < 16777216.f;
     }
@@ -184,7 +184,7 @@ __device__ __forceinline__ void add(Sums &s, float x, float c) {
 }
 
 // Two elements at a time, z by one packed FMA. nmc: -m c rounded once; what
-// that rounding shifts every z by (packed_pass keeps it to one) is put right
+// that rounding shifts every z by (packed_pass keeps it to a half) is put right
 // at the end of each batch.
 struct Sums2 {
     uint64_t l, t;
